@@ -58,7 +58,14 @@ extern "C" {
 #define MOLLA_ROW_SLOW_PATH 0x040u      /* informational: a sequential fallback ran for this row */
 #define MOLLA_ROW_DEGENERATE 0x080u     /* more equal values than the candidate buffer holds; token = -1 */
 #define MOLLA_ROW_SHARD_OVERFLOW 0x100u /* vocab-sharded form: a shard's list outgrew the exchange buffer */
-#define MOLLA_ROW_EMPTY 0x200u          /* the grammar mask left no candidate; token = -1 (the reference raises, sample.mojo:578-579) */
+#define MOLLA_ROW_EMPTY 0x200u          /* the grammar mask left no candidate; token = -1 (the reference raises, sample.mojo:578-579);
+                                         * in the losses: no logit of the row is above -inf */
+#define MOLLA_ROW_BAD_TOKEN 0x400u      /* losses: a token id outside the vocabulary (-1 apart, which means: no token) */
+
+/* Types of a block of logits, where a call takes more than fp32 */
+#define MOLLA_LOGITS_FP32 0
+#define MOLLA_LOGITS_BF16 1
+#define MOLLA_LOGITS_FP16 2
 
 /* Replaces nothing in the reference; lets a binding check what it loaded. */
 int32_t molla_sample_abi_version(void);
@@ -380,6 +387,83 @@ int32_t molla_sample_sharded_step(void *comm, int32_t rank, int32_t world, const
                                   const uint64_t *d_seed, const uint64_t *d_drawn, int32_t list_cap,
                                   void *d_workspace, int64_t workspace_bytes, void *stream, int32_t *d_tokens,
                                   uint32_t *d_row_status, float *d_diag, int64_t *wire_bytes);
+
+/* ---- what is trained on sampled tokens --------------------------------------------------------
+ * Logprobs of given tokens with their gradient, and two losses over them with theirs. No counterpart in
+ * the reference, which serves and does not train; they start where it stops: the tokens that
+ * `Sampler.pick` chose and the logprobs `Sampler.logprobs` gives them (src/molla/engine/sample.mojo:268-359).
+ *
+ * All of them read a block of B rows of V logits of type `logits_type` (MOLLA_LOGITS_*), row r at
+ * d_logits + r*row_stride elements, at most 720896 logits a row, and one token a row, d_tokens [B] int32, as
+ * molla_sample_batch leaves them. With z = logits / temperature of the row (d_temperature [B], NULL = 1;
+ * it has to be finite and above zero) the distribution of a row is softmax(z),
+ *     logprob = z[token] - ln sum exp z          entropy = - sum p ln p      (p ln p = 0 at p = 0)
+ *
+ * A row with token -1 has no token: it is not read, its logprob and entropy are 0 and its gradient is zeros.
+ * A row that cannot be answered says so in d_row_status (MOLLA_ROW_BAD_TOKEN, _EMPTY, _INVALID_CONFIG for
+ * its temperature, _LOAD_TIMEOUT): its logprob and entropy are NaN, and so is a loss it has a part in; its
+ * gradient is zeros. Logits of -inf, or of their type's lowest value, are ordinary values with p = 0; a NaN or +inf
+ * makes everything of its row NaN, the gradient too.
+ *
+ * d_grad_logits (NULL = not wanted) takes the gradient in the logits' type, rows grad_stride elements apart. It
+ * may be the logits themselves (same address, same stride), which are then overwritten; any other overlap is refused.
+ * Gradient rows whose factor is zero are zeros without the logits being read, whatever they hold.
+ *
+ * Everything within a row is held in 32 bits or more, sums over rows in 64 bits, each in an order of its own that
+ * does not depend on timing: the same call gives the same bits again. A row's logprob does not depend on
+ * the other rows or their number, and is the same from all these calls (rows of the same alignment to 16 bytes). */
+
+/* The logprobs of given tokens. d_logprob [B] and d_row_status [B] are required, d_entropy [B] may be NULL,
+ * and so may d_stats [B x 2], what the backward form wants: the row's maximum logit and its sum of
+ * exp((logit - maximum) / temperature). */
+int32_t molla_sample_token_logprobs(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V,
+                                    const int32_t *d_tokens, const float *d_temperature, void *stream, float *d_logprob,
+                                    float *d_entropy, float *d_stats, uint32_t *d_row_status);
+
+/* The gradient of any loss of those: d_grad_logprob [B] and d_grad_entropy [B] (NULL = none) are its derivatives by
+ * a row's logprob and entropy; d_entropy is needed with the latter. A row whose derivatives are both zero, or whose
+ * stats are those of a row without an answer, gets zeros. */
+int32_t molla_sample_token_logprobs_backward(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B,
+                                             int32_t V, const int32_t *d_tokens, const float *d_temperature,
+                                             const float *d_stats, const float *d_entropy, const float *d_grad_logprob,
+                                             const float *d_grad_entropy, void *stream, void *d_grad_logits,
+                                             int64_t grad_stride);
+
+/* The clipped policy loss with a KL term, and its gradient, in one call. With ratio = exp(logprob - old_logprob) and
+ * q = ref_logprob - logprob a row's loss is
+ *     weight * ( -min(ratio * advantage, clamp(ratio, 1 - clip_low, 1 + clip_high) * advantage)
+ *                + kl_coef * (exp(q) - q - 1) - entropy_coef * entropy )
+ * and the loss is scale * their sum; the gradient is of grad_scale * loss. d_weight [B] (NULL = 1) carries masks and the
+ * lengths of sequences, scale the number of tokens or sequences of all micro-batches and ranks. A row of weight 0 is treated as one without a token.
+ * d_ref_logprob [B] may be NULL when kl_coef is 0. At the clip's borders the gradient is the unclipped one.
+ * Outputs: d_loss [1], d_row_loss [B], d_logprob [B], d_row_status [B]; and, or NULL, d_entropy [B], d_kl [B] (the
+ * bracket of kl_coef; needs d_ref_logprob), d_clipped [B] (1 where the clip took the gradient away). */
+int32_t molla_sample_policy_loss(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V,
+                                 const int32_t *d_tokens, const float *d_temperature, const float *d_old_logprob,
+                                 const float *d_advantage, const float *d_weight, const float *d_ref_logprob,
+                                 float clip_low, float clip_high, float kl_coef, float entropy_coef, float scale,
+                                 float grad_scale, void *stream, float *d_loss, float *d_row_loss, float *d_logprob,
+                                 float *d_entropy, float *d_kl, uint8_t *d_clipped, void *d_grad_logits,
+                                 int64_t grad_stride, uint32_t *d_row_status);
+
+/* The preference loss over n_pairs pairs of a chosen and a rejected sequence, and its gradient, in one call.
+ * Sequence s is the rows d_seq_off[s] .. d_seq_off[s+1] (2 n_pairs + 1 offsets, which do not decrease, within 0..B);
+ * pair p is sequence 2p, chosen, and 2p+1, rejected; rows of no sequence take no part. With
+ *     seq_logratio[s] = sum over the rows of s that have a token of logprob - ref_logprob      (NULL = 0)
+ *     margin[p] = beta * (seq_logratio[2p] - seq_logratio[2p+1])
+ * a pair's loss is pair_weight[p] (NULL = 1) * ( -(1 - label_smoothing) ln sigmoid(margin) - label_smoothing ln sigmoid(-margin) )
+ * and the loss is scale * their sum; the gradient is of grad_scale * loss. label_smoothing is 0 to 0.5.
+ * Outputs: d_loss [1], d_logprob [B], d_row_status [B], d_pair_loss [n_pairs], d_margin [n_pairs], d_seq_logratio [2 n_pairs],
+ * d_pair_status [n_pairs] (what has no elements may be NULL): the error bits of the pair's rows, MOLLA_ROW_INVALID_CONFIG for offsets against the rules (then of no
+ * pair anything is computed: all losses are NaN and the gradient is zeros). A pair with such a status, or of weight 0, adds nothing to the gradient. */
+int64_t molla_sample_preference_workspace_bytes(int32_t B);
+int32_t molla_sample_preference_loss(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V,
+                                     const int32_t *d_tokens, const float *d_temperature, const int32_t *d_seq_off,
+                                     int32_t n_pairs, const float *d_ref_logprob, const float *d_pair_weight, float beta,
+                                     float label_smoothing, float scale, float grad_scale, void *d_workspace,
+                                     int64_t workspace_bytes, void *stream, float *d_loss, float *d_pair_loss,
+                                     float *d_margin, float *d_seq_logratio, float *d_logprob, void *d_grad_logits,
+                                     int64_t grad_stride, uint32_t *d_row_status, uint32_t *d_pair_status);
 
 /* cudaStreamSynchronize on `stream`, returning a status; then, if
  * `d_row_status` is given, nothing else is implied: rows report for themselves. */

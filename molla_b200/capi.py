@@ -28,8 +28,10 @@ ROW_SLOW_PATH = 0x040
 ROW_DEGENERATE = 0x080
 ROW_SHARD_OVERFLOW = 0x100
 ROW_EMPTY = 0x200
+ROW_BAD_TOKEN = 0x400
 ROW_TIE_BITS = ROW_TOPK_TIE | ROW_TOPP_TIE | ROW_CHOSEN_TIE
-ROW_ERROR_BITS = ROW_INVALID_CONFIG | ROW_UNSUPPORTED | ROW_LOAD_TIMEOUT | ROW_DEGENERATE | ROW_SHARD_OVERFLOW | ROW_EMPTY
+ROW_ERROR_BITS = ROW_INVALID_CONFIG | ROW_UNSUPPORTED | ROW_LOAD_TIMEOUT | ROW_DEGENERATE | ROW_SHARD_OVERFLOW | ROW_EMPTY | ROW_BAD_TOKEN
+LOGITS_FP32, LOGITS_BF16, LOGITS_FP16 = 0, 1, 2
 
 EXPORTS = (
     "molla_sample_abi_version", "molla_sample_last_error", "molla_sample_draw",
@@ -39,6 +41,8 @@ EXPORTS = (
     "molla_sample_pick_workspace_bytes", "molla_sample_pick_rows", "molla_sample_decode_step", "molla_sample_logprobs", "molla_sample_expf", "molla_sample_logf", "molla_sample_sync",
     "molla_sample_nccl_unique_id", "molla_sample_nccl_comm_create", "molla_sample_nccl_comm_destroy",
     "molla_sample_sharded_last_error", "molla_sample_sharded_workspace_bytes", "molla_sample_sharded_step",
+    "molla_sample_token_logprobs", "molla_sample_token_logprobs_backward", "molla_sample_policy_loss",
+    "molla_sample_preference_workspace_bytes", "molla_sample_preference_loss",
 )
 TESTING_EXPORTS = ("molla_sample_debug_knobs", "molla_sample_debug_profile", "molla_sample_debug_topk", "molla_sample_debug_launches",
                    "molla_sample_debug_softcap", "molla_sample_debug_softcap_quotients")
@@ -147,6 +151,17 @@ def _load(path, testing):
     L.molla_sample_sharded_step.restype = i32
     L.molla_sample_sharded_step.argtypes = ([vp, i32, i32, vp, i64, i32, i32, i32, i32] + [vp] * 16
                                             + [i32, vp, i64, vp, vp, vp, vp, vp])
+    block = [vp, i32, i64, i32, i32, vp, vp]   # logits, type, stride, rows, vocabulary, tokens, temperatures
+    L.molla_sample_token_logprobs.restype = i32
+    L.molla_sample_token_logprobs.argtypes = block + [vp] * 5
+    L.molla_sample_token_logprobs_backward.restype = i32
+    L.molla_sample_token_logprobs_backward.argtypes = block + [vp] * 6 + [i64]
+    L.molla_sample_policy_loss.restype = i32
+    L.molla_sample_policy_loss.argtypes = block + [vp] * 4 + [f32] * 6 + [vp] * 8 + [i64, vp]
+    L.molla_sample_preference_workspace_bytes.restype = i64
+    L.molla_sample_preference_workspace_bytes.argtypes = [i32]
+    L.molla_sample_preference_loss.restype = i32
+    L.molla_sample_preference_loss.argtypes = block + [vp, i32, vp, vp] + [f32] * 4 + [vp, i64] + [vp] * 7 + [i64, vp, vp]
     if testing:
         L.molla_sample_debug_knobs.restype = None
         L.molla_sample_debug_knobs.argtypes = [i32]

@@ -1,0 +1,35 @@
+// Logprobs of given tokens and the losses over them (molla_loss.cu), called by the entry points in molla_sample.cu.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+// A block of logits and what every one of these calls says about it.
+struct LossArgs {
+    const void *logits; int type; long long row_stride; int B, V;
+    const int *tokens; const float *temperature;
+    // outputs of a row (any but `logprob` and `status` may be nullptr)
+    float *logprob; float *entropy; float *stats; unsigned int *status;
+    // the gradient in the logits' type, or nullptr
+    void *grad; long long grad_stride;
+    // the row's derivatives, where they are given: by logprob (nullptr = the policy loss has them) and by entropy
+    const float *g_logprob; const float *g_entropy; const float *in_stats; const float *in_entropy;
+    // the policy loss
+    const float *old_logprob; const float *advantage; const float *weight; const float *ref_logprob;
+    float clip_low, clip_high, kl_coef, entropy_coef, scale, grad_scale;
+    float *loss; float *row_loss; float *kl; unsigned char *clipped;
+};
+
+// The preference loss between its two passes over the logits.
+struct PairArgs {
+    int B, n_pairs;
+    const int *tokens; const int *off; const float *logprob; const float *ref_logprob; const float *weight; const unsigned int *row_status;
+    float beta, smoothing, scale, grad_scale;
+    float *loss; float *pair_loss; float *margin; float *seq_logratio; unsigned int *pair_status;
+    float *g_logprob;            // [B] the rows' derivatives, or nullptr
+};
+
+cudaError_t molla_loss_score(const LossArgs &a, cudaStream_t st);      // logprobs, entropies, stats
+cudaError_t molla_loss_backward(const LossArgs &a, cudaStream_t st);   // the gradient from stats and the rows' derivatives
+cudaError_t molla_loss_policy(const LossArgs &a, cudaStream_t st);     // the policy loss and its gradient
+cudaError_t molla_loss_pairs(const PairArgs &a, cudaStream_t st);

@@ -50,6 +50,7 @@
 #include "molla_exact.cuh"
 #include "molla_cluster.h"
 #include "molla_logprob.h"
+#include "molla_loss.h"
 #include "molla_rows.h"
 
 using namespace molla;
@@ -1810,6 +1811,35 @@ int launch_logprobs(const float *logits, int64_t row_stride, int B, int V, const
     return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "logprob launch failed: %s", cudaGetErrorString(e));
 }
 
+// ---- the losses: the block of logits of a call, and the gradient's place
+
+int loss_block(LossArgs &a, const void *logits, int type, int64_t row_stride, int B, int V, const int *tokens, const float *temperature) {
+    if (!logits || !tokens) return fail(MOLLA_ERR_ARGUMENT, "logits and tokens are required%s");
+    if (type != MOLLA_LOGITS_FP32 && type != MOLLA_LOGITS_BF16 && type != MOLLA_LOGITS_FP16) return fail(MOLLA_ERR_ARGUMENT, "logits are fp32, bf16 or fp16%s");
+    if (B < 0 || V <= 0 || row_stride < V) return fail(MOLLA_ERR_ARGUMENT, "bad block shape%s");
+    if (V > MAX_VOCAB) return fail(MOLLA_ERR_VOCAB, "vocabulary too wide%s");
+    if ((uintptr_t)logits % (type == MOLLA_LOGITS_FP32 ? 4 : 2)) return fail(MOLLA_ERR_ARGUMENT, "logits have to be aligned to their type%s");
+    a.logits = logits; a.type = type; a.row_stride = row_stride; a.B = B; a.V = V;
+    a.tokens = tokens; a.temperature = temperature;
+    return MOLLA_OK;
+}
+
+int loss_gradient(LossArgs &a, void *grad, int64_t stride) {
+    const int64_t size = a.type == MOLLA_LOGITS_FP32 ? 4 : 2;
+    if (stride < a.V) return fail(MOLLA_ERR_ARGUMENT, "bad stride of the gradient%s");
+    if ((uintptr_t)grad % size) return fail(MOLLA_ERR_ARGUMENT, "the gradient has to be aligned to its type%s");
+    // In the logits' place or clear of them: rows may interleave only where both have the same stride.
+    const int64_t x = (int64_t)(uintptr_t)a.logits, g = (int64_t)(uintptr_t)grad, row = (int64_t)a.V * size;
+    if (a.B > 0 && !(x == g && stride == a.row_stride)) {
+        const int64_t x_end = x + (int64_t)(a.B - 1) * a.row_stride * size + row, g_end = g + (int64_t)(a.B - 1) * stride * size + row;
+        const int64_t step = stride * size, by = ((g - x) % step + step) % step;
+        const bool interleaved = stride == a.row_stride && by >= row && step - by >= row;
+        if (x < g_end && g < x_end && !interleaved) return fail(MOLLA_ERR_ARGUMENT, "the gradient overlaps the logits without taking their place%s");
+    }
+    a.grad = grad; a.grad_stride = stride;
+    return MOLLA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -2526,6 +2556,110 @@ int64_t molla_sample_debug_softcap_quotients(void) {
     return e == cudaSuccess ? (int64_t)n : -1;
 }
 #endif
+
+// ---- logprobs of given tokens and the losses over them (molla_loss.cu)
+
+int32_t molla_sample_token_logprobs(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V,
+                                    const int32_t *d_tokens, const float *d_temperature, void *stream, float *d_logprob,
+                                    float *d_entropy, float *d_stats, uint32_t *d_row_status) {
+    g_err[0] = 0;
+    LossArgs a = {};
+    const int rc = loss_block(a, d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature);
+    if (rc != MOLLA_OK) return rc;
+    if (!d_logprob || !d_row_status) return fail(MOLLA_ERR_ARGUMENT, "logprobs and row status are required%s");
+    a.logprob = d_logprob; a.entropy = d_entropy; a.stats = d_stats; a.status = d_row_status;
+    const cudaError_t e = molla_loss_score(a, (cudaStream_t)stream);
+    return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "logprob launch failed: %s", cudaGetErrorString(e));
+}
+
+int32_t molla_sample_token_logprobs_backward(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B,
+                                             int32_t V, const int32_t *d_tokens, const float *d_temperature,
+                                             const float *d_stats, const float *d_entropy, const float *d_grad_logprob,
+                                             const float *d_grad_entropy, void *stream, void *d_grad_logits,
+                                             int64_t grad_stride) {
+    g_err[0] = 0;
+    LossArgs a = {};
+    int rc = loss_block(a, d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature);
+    if (rc != MOLLA_OK) return rc;
+    if (!d_stats || !d_grad_logprob || !d_grad_logits) return fail(MOLLA_ERR_ARGUMENT, "stats, the derivatives by the logprobs and the gradient are required%s");
+    if (d_grad_entropy && !d_entropy) return fail(MOLLA_ERR_ARGUMENT, "derivatives by the entropies need the entropies%s");
+    rc = loss_gradient(a, d_grad_logits, grad_stride);
+    if (rc != MOLLA_OK) return rc;
+    a.in_stats = d_stats; a.in_entropy = d_entropy; a.g_logprob = d_grad_logprob; a.g_entropy = d_grad_entropy;
+    const cudaError_t e = molla_loss_backward(a, (cudaStream_t)stream);
+    return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "gradient launch failed: %s", cudaGetErrorString(e));
+}
+
+int32_t molla_sample_policy_loss(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V,
+                                 const int32_t *d_tokens, const float *d_temperature, const float *d_old_logprob,
+                                 const float *d_advantage, const float *d_weight, const float *d_ref_logprob,
+                                 float clip_low, float clip_high, float kl_coef, float entropy_coef, float scale,
+                                 float grad_scale, void *stream, float *d_loss, float *d_row_loss, float *d_logprob,
+                                 float *d_entropy, float *d_kl, uint8_t *d_clipped, void *d_grad_logits,
+                                 int64_t grad_stride, uint32_t *d_row_status) {
+    g_err[0] = 0;
+    LossArgs a = {};
+    int rc = loss_block(a, d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature);
+    if (rc != MOLLA_OK) return rc;
+    if (!d_old_logprob || !d_advantage) return fail(MOLLA_ERR_ARGUMENT, "old logprobs and advantages are required%s");
+    if (!d_loss || !d_row_loss || !d_logprob || !d_row_status) return fail(MOLLA_ERR_ARGUMENT, "loss, row losses, logprobs and row status are required%s");
+    if (!(clip_low >= 0.0f) || !(clip_high >= 0.0f)) return fail(MOLLA_ERR_CONFIG, "a clip range cannot be negative%s");
+    if (!isfinite(kl_coef) || !isfinite(entropy_coef)) return fail(MOLLA_ERR_CONFIG, "the coefficients of KL and entropy have to be finite%s");
+    if (!isfinite(scale) || !isfinite(grad_scale)) return fail(MOLLA_ERR_CONFIG, "the scales of loss and gradient have to be finite%s");
+    if ((kl_coef != 0.0f || d_kl) && !d_ref_logprob) return fail(MOLLA_ERR_ARGUMENT, "a KL term needs reference logprobs%s");
+    if (d_grad_logits && (rc = loss_gradient(a, d_grad_logits, grad_stride)) != MOLLA_OK) return rc;
+    a.old_logprob = d_old_logprob; a.advantage = d_advantage; a.weight = d_weight; a.ref_logprob = d_ref_logprob;
+    a.clip_low = clip_low; a.clip_high = clip_high; a.kl_coef = kl_coef; a.entropy_coef = entropy_coef;
+    a.scale = scale; a.grad_scale = grad_scale;
+    a.loss = d_loss; a.row_loss = d_row_loss; a.logprob = d_logprob; a.entropy = d_entropy; a.kl = d_kl; a.clipped = d_clipped;
+    a.status = d_row_status;
+    const cudaError_t e = molla_loss_policy(a, (cudaStream_t)stream);
+    return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "policy loss launch failed: %s", cudaGetErrorString(e));
+}
+
+int64_t molla_sample_preference_workspace_bytes(int32_t B) {
+    if (B < 0) return fail(MOLLA_ERR_ARGUMENT, "bad shape for the workspace query%s");
+    return (((int64_t)B * 12 + 255) / 256 + 1) * 256;   // the rows' stats and derivatives
+}
+
+int32_t molla_sample_preference_loss(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V,
+                                     const int32_t *d_tokens, const float *d_temperature, const int32_t *d_seq_off,
+                                     int32_t n_pairs, const float *d_ref_logprob, const float *d_pair_weight, float beta,
+                                     float label_smoothing, float scale, float grad_scale, void *d_workspace,
+                                     int64_t workspace_bytes, void *stream, float *d_loss, float *d_pair_loss,
+                                     float *d_margin, float *d_seq_logratio, float *d_logprob, void *d_grad_logits,
+                                     int64_t grad_stride, uint32_t *d_row_status, uint32_t *d_pair_status) {
+    g_err[0] = 0;
+    LossArgs a = {};
+    int rc = loss_block(a, d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature);
+    if (rc != MOLLA_OK) return rc;
+    if (n_pairs < 0 || n_pairs > (1 << 30) - 1) return fail(MOLLA_ERR_ARGUMENT, "bad number of pairs%s");
+    if (!d_seq_off) return fail(MOLLA_ERR_ARGUMENT, "sequence offsets are required%s");
+    if (!d_loss || !d_logprob || !d_row_status || (n_pairs > 0 && (!d_pair_loss || !d_margin || !d_seq_logratio || !d_pair_status)))
+        return fail(MOLLA_ERR_ARGUMENT, "loss, pair losses, margins, log ratios, logprobs and status words are required%s");
+    if (!(beta > 0.0f) || isinf(beta)) return fail(MOLLA_ERR_CONFIG, "beta has to be finite and above zero%s");
+    if (!(label_smoothing >= 0.0f && label_smoothing <= 0.5f)) return fail(MOLLA_ERR_CONFIG, "label smoothing has to be between zero and a half%s");
+    if (!isfinite(scale) || !isfinite(grad_scale)) return fail(MOLLA_ERR_CONFIG, "the scales of loss and gradient have to be finite%s");
+    if (!d_workspace || workspace_bytes < molla_sample_preference_workspace_bytes(B))
+        return fail(MOLLA_ERR_WORKSPACE, "workspace missing or too small%s");
+    if ((uintptr_t)d_workspace % 8) return fail(MOLLA_ERR_ARGUMENT, "the workspace has to start on a multiple of 8 bytes%s");
+    if (d_grad_logits && (rc = loss_gradient(a, d_grad_logits, grad_stride)) != MOLLA_OK) return rc;
+    float *stats = (float *)d_workspace, *g = stats + 2 * (int64_t)B;
+    LossArgs score = a;
+    score.grad = nullptr;
+    score.logprob = d_logprob; score.status = d_row_status; score.stats = stats;
+    cudaError_t e = molla_loss_score(score, (cudaStream_t)stream);
+    PairArgs p = {};
+    p.B = B; p.n_pairs = n_pairs; p.tokens = d_tokens; p.off = d_seq_off; p.logprob = d_logprob; p.ref_logprob = d_ref_logprob;
+    p.weight = d_pair_weight; p.row_status = d_row_status;
+    p.beta = beta; p.smoothing = label_smoothing; p.scale = scale; p.grad_scale = grad_scale;
+    p.loss = d_loss; p.pair_loss = d_pair_loss; p.margin = d_margin; p.seq_logratio = d_seq_logratio; p.pair_status = d_pair_status;
+    p.g_logprob = d_grad_logits ? g : nullptr;
+    if (e == cudaSuccess) e = molla_loss_pairs(p, (cudaStream_t)stream);
+    a.in_stats = stats; a.g_logprob = g;
+    if (e == cudaSuccess && d_grad_logits) e = molla_loss_backward(a, (cudaStream_t)stream);
+    return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "preference loss launch failed: %s", cudaGetErrorString(e));
+}
 
 int32_t molla_sample_sync(void *stream) {
     cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
