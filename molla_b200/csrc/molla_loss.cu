@@ -13,11 +13,21 @@
 #include <stdint.h>
 
 #include "../../include/molla_sample.h"
+#include "molla_device.cuh"
 #include "molla_loss.h"
+
+using namespace molla;
+
+#ifdef MOLLA_SAMPLE_TESTING
+#define LOSS_KNOB(a, bit) (((a).knobs & (bit)) != 0)
+#else
+#define LOSS_KNOB(a, bit) false
+#endif
 
 namespace {
 
-constexpr float LOG2E = 1.44269504088896340736f;
+constexpr double LOG2E_64 = 1.44269504088896340736;
+constexpr float LOG2E = (float)LOG2E_64;
 constexpr float DEEP = -1e30f;    // where x - M is held, so that 0 * (x - M) is 0 for logits of -inf too
 constexpr unsigned int ROW_ERRORS = MOLLA_ROW_BAD_TOKEN | MOLLA_ROW_EMPTY | MOLLA_ROW_INVALID_CONFIG | MOLLA_ROW_LOAD_TIMEOUT;
 
@@ -62,9 +72,9 @@ __device__ __forceinline__ RowIn row_in(const LossArgs &a, int r) {
 // The gradient's three numbers: add at the token, and A and H of the formula.
 struct RowGrad { float token, A, H; };
 
-__device__ __forceinline__ RowGrad row_grad(double g, double h, float T, float S, double w_over_st) {
+__device__ __forceinline__ RowGrad row_grad(double g, double h, float T, double S, double w_over_st) {
     RowGrad o;
-    const double inv = 1.0 / ((double)T * (double)S);
+    const double inv = 1.0 / ((double)T * S);
     o.token = (float)(g / (double)T);
     o.A = (float)((g - h * w_over_st) * inv);
     o.H = (float)(h * inv / (double)T);
@@ -72,36 +82,40 @@ __device__ __forceinline__ RowGrad row_grad(double g, double h, float T, float S
 }
 
 // What a row answers once its maximum M, sum S and, where entropies are wanted, W are known. One thread.
-__device__ RowGrad row_answer(const LossArgs &a, int r, const RowIn &in, float xt, float M, float S, float W) {
-    const bool empty = M == -INFINITY;
-    const unsigned int status = in.status | (empty && !in.status ? MOLLA_ROW_EMPTY : 0u);
-    const double T = in.T, lnS = log((double)S);
+__device__ RowGrad row_answer(const LossArgs &a, int r, const RowIn &in, float xt, float M, double S, double W, float c, bool write) {
+    const unsigned int status = in.status | (M == -INFINITY && S == 0.0 && !in.status ? MOLLA_ROW_EMPTY : 0u);
+    // ln p in the temperature that c stands for (log2(e)/T rounded): the error of c then moves ln S and the token together
+    const double T = LOG2E_64 / (double)c, lnS = log(S);
     const double l = ((double)xt - (double)M) / T - lnS;
     const bool want_entropy = a.entropy != nullptr || a.entropy_coef != 0.0f;
-    const double w_over_st = want_entropy ? (double)W / ((double)S * T) : 0.0;
+    const double w_over_st = want_entropy ? W / (S * T) : 0.0;
     const double H = lnS - w_over_st;
     RowGrad o{0.0f, 0.0f, 0.0f};
-    a.status[r] = status;
-    a.logprob[r] = status ? NAN : (float)l;
-    if (a.entropy) a.entropy[r] = status ? NAN : (float)H;
-    if (a.stats) { a.stats[2 * r] = status ? NAN : M; a.stats[2 * r + 1] = status ? 0.0f : S; }
+    if (write) {
+        a.status[r] = status;
+        a.logprob[r] = status ? NAN : (float)l;
+        if (a.entropy) a.entropy[r] = status ? NAN : (float)H;
+        if (a.stats) { a.stats[2 * r] = status ? NAN : M; a.stats[2 * r + 1] = status ? 0.0f : (float)S; }
+    }
     if (!a.row_loss) return o;
     // the policy loss
     const double w = a.weight ? (double)a.weight[r] : 1.0;
     const double ratio = exp(l - (double)a.old_logprob[r]), adv = a.advantage[r];
     const double lo = 1.0 - (double)a.clip_low, hi = 1.0 + (double)a.clip_high;
-    const double u = ratio * adv, c = fmin(fmax(ratio, lo), hi) * adv;
-    const bool held = c < u;
-    double term = -(held ? c : u), g = held ? 0.0 : -u;   // (a ratio that is NaN is not held)
+    const double u = ratio * adv, v = fmin(fmax(ratio, lo), hi) * adv;
+    const bool held = v < u;
+    double term = -(held ? v : u), g = held ? 0.0 : -u;   // (a ratio that is NaN is not held)
     if (a.ref_logprob) {
         const double q = (double)a.ref_logprob[r] - l, eq = expm1(q), kl = eq - q;
-        if (a.kl) a.kl[r] = status ? NAN : (float)kl;
+        if (a.kl && write) a.kl[r] = status ? NAN : (float)kl;
         if (a.kl_coef != 0.0f) { term += (double)a.kl_coef * kl; g -= (double)a.kl_coef * eq; }
     }
     double h = 0.0;
     if (a.entropy_coef != 0.0f) { term -= (double)a.entropy_coef * H; h = -w * (double)a.entropy_coef; }
-    a.row_loss[r] = status ? NAN : (float)(w * term);
-    if (a.clipped) a.clipped[r] = !status && held;
+    if (write) {
+        a.row_loss[r] = status ? NAN : (float)(w * term);
+        if (a.clipped) a.clipped[r] = !status && held;
+    }
     const double gs = (double)a.scale * (double)a.grad_scale;
     if (!status) o = row_grad(g * w * gs, h * gs, in.T, S, w_over_st);
     return o;
@@ -117,92 +131,508 @@ __device__ void row_idle(const LossArgs &a, int r) {
     if (a.clipped) a.clipped[r] = 0;
 }
 
-// ---- a block a row --------------------------------------------------------------------------------
+// ---- packed pairs, and a 16-byte chunk of logits -----------------------------------------------------
 
-constexpr int NT = 512;
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) { f32x2 v; asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); return v; }
+__device__ __forceinline__ void unpack2(f32x2 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 v; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b)); return v; }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 v; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b)); return v; }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 v; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c)); return v; }
 
-__device__ float block_max(float v, float *ws) {
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, i));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float m = ws[0];
-    for (int i = 1; i < NT / 32; i++) m = fmaxf(m, ws[i]);
-    return m;
+template <class T> struct Chunk;
+template <> struct Chunk<float> {
+    static constexpr int N = 4;
+    __device__ static __forceinline__ f32x2 pair(const uint4 &v, int i) {
+        return i == 0 ? pack2(__uint_as_float(v.x), __uint_as_float(v.y)) : pack2(__uint_as_float(v.z), __uint_as_float(v.w));
+    }
+    __device__ static __forceinline__ float most(const uint4 &v) {
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    }
+    __device__ static __forceinline__ uint4 most2(const uint4 &a, const uint4 &b) {
+        return make_uint4(m(a.x, b.x), m(a.y, b.y), m(a.z, b.z), m(a.w, b.w));
+    }
+    __device__ static __forceinline__ unsigned int m(unsigned int a, unsigned int b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+    __device__ static __forceinline__ void put(uint4 &o, int i, float lo, float hi) {
+        if (i == 0) { o.x = __float_as_uint(lo); o.y = __float_as_uint(hi); } else { o.z = __float_as_uint(lo); o.w = __float_as_uint(hi); }
+    }
+    static constexpr unsigned int LOWEST = 0xff800000u;   // -inf
+};
+__device__ __forceinline__ unsigned int word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ void set_word(uint4 &v, int i, unsigned int w) { if (i == 0) v.x = w; else if (i == 1) v.y = w; else if (i == 2) v.z = w; else v.w = w; }
+template <> struct Chunk<__nv_bfloat16> {
+    static constexpr int N = 8;
+    __device__ static __forceinline__ f32x2 pair(const uint4 &v, int i) {
+        const unsigned int w = word(v, i);
+        return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+    __device__ static __forceinline__ unsigned int m(unsigned int a, unsigned int b) {
+        const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+        return *reinterpret_cast<const unsigned int *>(&r);
+    }
+    __device__ static __forceinline__ uint4 most2(const uint4 &a, const uint4 &b) { return make_uint4(m(a.x, b.x), m(a.y, b.y), m(a.z, b.z), m(a.w, b.w)); }
+    __device__ static __forceinline__ float most(const uint4 &v) {
+        const unsigned int w = m(m(v.x, v.y), m(v.z, v.w));
+        return fmaxf(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+    __device__ static __forceinline__ void put(uint4 &o, int i, float lo, float hi) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+        set_word(o, i, *reinterpret_cast<const unsigned int *>(&r));
+    }
+    static constexpr unsigned int LOWEST = 0xff80ff80u;
+};
+template <> struct Chunk<__half> {
+    static constexpr int N = 8;
+    __device__ static __forceinline__ f32x2 pair(const uint4 &v, int i) {
+        const unsigned int w = word(v, i);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        return pack2(f.x, f.y);
+    }
+    __device__ static __forceinline__ unsigned int m(unsigned int a, unsigned int b) {
+        const __half2 r = __hmax2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+        return *reinterpret_cast<const unsigned int *>(&r);
+    }
+    __device__ static __forceinline__ uint4 most2(const uint4 &a, const uint4 &b) { return make_uint4(m(a.x, b.x), m(a.y, b.y), m(a.z, b.z), m(a.w, b.w)); }
+    __device__ static __forceinline__ float most(const uint4 &v) {
+        const unsigned int w = m(m(v.x, v.y), m(v.z, v.w));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        return fmaxf(f.x, f.y);
+    }
+    __device__ static __forceinline__ void put(uint4 &o, int i, float lo, float hi) {
+        const __half2 r = __floats2half2_rn(lo, hi);
+        set_word(o, i, *reinterpret_cast<const unsigned int *>(&r));
+    }
+    static constexpr unsigned int LOWEST = 0xfc00fc00u;
+};
+
+// ---- rows by clusters, a unit of 1024 logits by a warp ------------------------------------------------
+
+constexpr int UNIT = 1024;
+constexpr int MAX_WARPS = 16;
+constexpr int WAIT_TRIES = 1 << 22;   // of a bounded wait
+
+// How a launch lays its rows out: C blocks of W warps a row, R units of shared memory a warp, `rows_at_once` rows
+// in flight. Nothing in a row's results depends on it: a unit is always one warp's, in the same order of additions, and
+// the units are put together in theirs.
+struct Layout { int C, W, R, rows_at_once, units; bool resident; };
+
+// The row's logits in memory: what lies before the first 16-byte boundary and behind the last (the edge, at most 14 logits), and
+// whole 16-byte chunks in between, in units.
+template <class T> struct RowSpan {
+    const T *x; int head, units, tail; int bytes;
+    __device__ __forceinline__ RowSpan(const T *row, int V) {
+        const int off = (int)((uintptr_t)row & 15);
+        head = off ? (16 - off) / (int)sizeof(T) : 0;
+        if (head > V) head = V;
+        x = row + head;
+        bytes = ((V - head) * (int)sizeof(T)) & ~15;
+        tail = V - head - bytes / (int)sizeof(T);
+        units = (bytes + UNIT * (int)sizeof(T) - 1) / (UNIT * (int)sizeof(T));
+    }
+    __device__ __forceinline__ int unit_bytes(int u) const { return min(bytes - u * UNIT * (int)sizeof(T), UNIT * (int)sizeof(T)); }
+    __device__ __forceinline__ bool edge() const { return head + tail > 0; }
+    // the edge's logit of a lane: the first lanes have the head, those from 16 on the tail; -1 if it has none
+    __device__ __forceinline__ int edge_at(int lane) const {
+        if (lane < head) return lane - head;
+        const int t = lane - 16;
+        return t >= 0 && t < tail ? bytes / (int)sizeof(T) + t : INT32_MIN;
+    }
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
-__device__ float block_sum(float v, float *ws) {
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) v += __shfl_xor_sync(0xffffffffu, v, i);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float s = ws[0];
-    for (int i = 1; i < NT / 32; i++) s += ws[i];
-    return s;
+    return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) v += __shfl_xor_sync(0xffffffffu, v, i);
+    return v;
 }
 
-template <class T>
-__device__ void write_gradient(const LossArgs &a, int r, const T *x, int token, float M, float c, const RowGrad &q, bool zero) {
-    T *out = (T *)a.grad + (long long)r * a.grad_stride;
-    for (int j = threadIdx.x; j < a.V; j += NT) {
-        float v = 0.0f;
-        if (!zero) {
-            const float raw = __fsub_rn(to_f32(x[j]), M), d = raw < DEEP ? DEEP : raw;
-            v = -ex2(d * c) * __fmaf_rn(q.H, d, q.A);
-            if (j == token) v += q.token;
+// 2^t for t <= 0 without ex2's bias: the nearest integer apart, the Taylor series of 2^f = e^(f ln 2) for the rest (|f| <= 1/2; the first term
+// left out is below 6e-9 of the sum).
+__device__ __forceinline__ float exp2_series(float t) {
+    if (!(t > -126.0f)) return t != t ? t : 0.0f;
+    const float n = rintf(t), f = __fmul_rn(t - n, 0.693147180559945f);
+    float p = 1.0f / 5040.0f;
+    p = __fmaf_rn(p, f, 1.0f / 720.0f); p = __fmaf_rn(p, f, 1.0f / 120.0f); p = __fmaf_rn(p, f, 1.0f / 24.0f);
+    p = __fmaf_rn(p, f, 1.0f / 6.0f); p = __fmaf_rn(p, f, 0.5f); p = __fmaf_rn(p, f, 1.0f); p = __fmaf_rn(p, f, 1.0f);
+    return p * __int_as_float(((int)n + 127) << 23);
+}
+
+// ex2.approx is low by 5.2e-8 in the mean, alike in every binade (4 million arguments from -32 to 0), which a sum of many terms
+// keeps: uncorrected, the log ratio of a sequence of 200 rows was off by 1e-5. Its value at 0 is exact.
+constexpr float EX2_LOW = 5.2e-8f;
+
+struct Stat { float m, s, w; unsigned int late; };   // maximum, sum, weighted sum of a unit; a wait that ran out
+
+template <class T, bool ENT>
+__device__ __forceinline__ Stat unit_stat(const uint4 (&v)[UNIT * sizeof(T) / 512], float c) {
+    constexpr int K = UNIT * sizeof(T) / 512, P = Chunk<T>::N / 2;
+    uint4 most = v[0];
+#pragma unroll
+    for (int i = 1; i < K; i++) most = Chunk<T>::most2(most, v[i]);
+    Stat o;
+    o.m = warp_max(Chunk<T>::most(most));
+    o.late = 0;
+    const float m = o.m == -INFINITY ? 0.0f : o.m;   // nothing but -inf (and NaN): sums of 0 (and NaN)
+    const f32x2 minus_m = pack2(-m, -m), cc = pack2(c, c);
+    f32x2 s = 0, w = 0;
+#pragma unroll
+    for (int i = 0; i < K; i++)
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            const f32x2 d = add2(Chunk<T>::pair(v[i], j), minus_m);
+            float lo, hi;
+            unpack2(mul2(d, cc), lo, hi);
+            const f32x2 e = pack2(ex2(lo), ex2(hi));
+            s = add2(s, e);
+            if (ENT) {
+                unpack2(d, lo, hi);
+                w = fma2(e, pack2(lo < DEEP ? DEEP : lo, hi < DEEP ? DEEP : hi), w);
+            }
         }
-        out[j] = from_f32<T>(v);
+    float lo, hi;
+    unpack2(s, lo, hi);
+    const float sum = warp_sum(lo + hi);
+    o.s = o.m == -INFINITY ? sum : __fmaf_rn(EX2_LOW, sum - 1.0f, sum);
+    o.w = 0.0f;
+    if (ENT) {
+        unpack2(w, lo, hi);
+        const float ws = warp_sum(lo + hi);
+        o.w = __fmaf_rn(EX2_LOW, ws, ws);
+    }
+    return o;
+}
+
+// The edge's, a logit a lane (-inf where there is none).
+template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) {
+    Stat o;
+    o.m = warp_max(x);
+    o.late = 0;
+    const float m = o.m == -INFINITY ? 0.0f : o.m, d = __fsub_rn(x, m), e = ex2(d * c), sum = warp_sum(e);
+    o.s = o.m == -INFINITY ? sum : __fmaf_rn(EX2_LOW, sum - 1.0f, sum);
+    o.w = ENT ? warp_sum(e * (d < DEEP ? DEEP : d)) : 0.0f;
+    return o;
+}
+
+// All units of a row: a warp, the units in turn over the lanes, in 64 bits.
+template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, double &S, double &W, unsigned int &late) {
+    const int lane = threadIdx.x & 31;
+    float m = -INFINITY;
+    unsigned int l = 0;
+    for (int u = lane; u < n; u += 32) { m = fmaxf(m, st[u].m); l |= st[u].late; }
+    M = warp_max(m);
+    late = __reduce_or_sync(0xffffffffu, l);
+    double s = 0.0, w = 0.0;
+    for (int u = lane; u < n; u += 32) {
+        const Stat o = st[u];
+        const float d = o.m == -INFINITY ? 0.0f : __fsub_rn(o.m, M);   // (a unit of -inf: sums of 0, or NaN)
+        const double f = (double)exp2_series(d * c);
+        s += f * (double)o.s;
+        if (ENT) w += f * ((double)o.w + (double)(d < DEEP ? DEEP : d) * (double)o.s);
+    }
+    S = warp_sum(s);
+    W = ENT ? warp_sum(w) : 0.0;
+}
+
+template <class T, bool ENT>
+__device__ __forceinline__ float gradient_of(float x, float M, float c, float A, float H) {
+    const float d = __fsub_rn(x, M), e = ex2(d * c);
+    return ENT ? -(e * __fmaf_rn(H, d < DEEP ? DEEP : d, A)) : -(e * A);
+}
+
+// One unit's gradient: `to` is where its first logit's goes.
+template <class T, bool ENT>
+__device__ __forceinline__ void unit_gradient(const uint4 *slot, int bytes, T *to, bool wide, float M, float c, float A, float H) {
+    constexpr int K = UNIT * sizeof(T) / 512, N = Chunk<T>::N;
+    const int lane = threadIdx.x & 31, chunks = bytes >> 4;
+    const f32x2 minus_M = pack2(-M, -M), cc = pack2(c, c), aa = pack2(-A, -A), hh = pack2(-H, -H);
+#pragma unroll
+    for (int i = 0; i < K; i++) {
+        const int k = i * 32 + lane;
+        if (k >= chunks) break;
+        const uint4 v = slot[k];
+        uint4 o;
+#pragma unroll
+        for (int j = 0; j < N / 2; j++) {
+            const f32x2 d = add2(Chunk<T>::pair(v, j), minus_M);
+            float lo, hi;
+            unpack2(mul2(d, cc), lo, hi);
+            const f32x2 e = pack2(ex2(lo), ex2(hi));
+            f32x2 g = aa;
+            if (ENT) {
+                unpack2(d, lo, hi);
+                g = fma2(hh, pack2(lo < DEEP ? DEEP : lo, hi < DEEP ? DEEP : hi), aa);
+            }
+            unpack2(mul2(e, g), lo, hi);
+            Chunk<T>::put(o, j, lo, hi);
+        }
+        if (wide) {
+            __stcs(reinterpret_cast<uint4 *>(to) + k, o);
+        } else {
+            const T *e = reinterpret_cast<const T *>(&o);
+#pragma unroll
+            for (int j = 0; j < N; j++) to[k * N + j] = e[j];
+        }
     }
 }
 
-// Everything a row's logits are read for: logprob, and with `a.grad` the policy loss's gradient.
-template <class T>
-__global__ void __launch_bounds__(NT) rows_kernel(const __grid_constant__ LossArgs a) {
-    __shared__ float ws[NT / 32];
-    __shared__ RowGrad s_grad;
-    const int r = blockIdx.x;
-    const T *x = (const T *)a.logits + (long long)r * a.row_stride;
-    const RowIn in = row_in(a, r);
-    float M = 0.0f, S = 1.0f, W = 0.0f;
-    const float c = LOG2E / in.T;
-    if (in.idle) {
-        if (threadIdx.x == 0) { row_idle(a, r); s_grad = RowGrad{0.0f, 0.0f, 0.0f}; }
-    } else {
-        if (!in.status) {
-            float m = -INFINITY;
-            for (int j = threadIdx.x; j < a.V; j += NT) m = fmaxf(m, to_f32(x[j]));
-            M = block_max(m, ws);
-            float s = 0.0f, w = 0.0f;
-            if (M > -INFINITY)
-                for (int j = threadIdx.x; j < a.V; j += NT) {
-                    const float raw = __fsub_rn(to_f32(x[j]), M), d = raw < DEEP ? DEEP : raw, e = ex2(d * c);
-                    s += e;
-                    w = __fmaf_rn(e, d, w);
-                }
-            S = block_sum(s, ws);
-            W = block_sum(w, ws);
-        }
-        if (threadIdx.x == 0) s_grad = row_answer(a, r, in, in.status ? 0.0f : to_f32(x[in.token]), M, S, W);
+__device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
+
+// A row of zeros, by the warps of its blocks.
+template <class T> __device__ void zero_row(T *out, int V, int warp, int warps) {
+    const int lane = threadIdx.x & 31;
+    const int off = (int)((uintptr_t)out & 15), head = min(off ? (16 - off) / (int)sizeof(T) : 0, V);
+    const int chunks = (V - head) / Chunk<T>::N, tail = V - head - chunks * Chunk<T>::N;
+    uint4 *to = reinterpret_cast<uint4 *>(out + head);
+    for (int k = warp * 32 + lane; k < chunks; k += warps * 32) __stcs(to + k, zero4());
+    if (warp == 0) {
+        if (lane < head) out[lane] = from_f32<T>(0.0f);
+        if (lane < tail) out[head + chunks * Chunk<T>::N + lane] = from_f32<T>(0.0f);
     }
-    if (!a.grad) return;
-    __syncthreads();
-    const RowGrad q = s_grad;
-    write_gradient<T>(a, r, x, in.token, M, c, q, q.token == 0.0f && q.A == 0.0f && q.H == 0.0f);
 }
 
-// The gradient from the stats of an earlier pass.
-template <class T>
-__global__ void __launch_bounds__(NT) backward_kernel(const __grid_constant__ LossArgs a) {
-    const int r = blockIdx.x;
-    const T *x = (const T *)a.logits + (long long)r * a.row_stride;
+// What a row's gradient is made of, where it is given (the backward pass).
+struct Given { bool zero; float M, c; RowGrad q; };
+__device__ __forceinline__ Given row_given(const LossArgs &a, int r) {
+    Given o;
     const int token = a.tokens[r];
-    const float temp = a.temperature ? a.temperature[r] : 1.0f, M = a.in_stats[2 * r], S = a.in_stats[2 * r + 1];
+    const float temp = a.temperature ? a.temperature[r] : 1.0f, S = a.in_stats[2 * r + 1];
     const float g = a.g_logprob[r], h = a.g_entropy ? a.g_entropy[r] : 0.0f;
-    const bool zero = token < 0 || token >= a.V || (g == 0.0f && h == 0.0f) || S == 0.0f;
-    RowGrad q{0.0f, 0.0f, 0.0f};
-    if (!zero) q = row_grad(g, h, temp, S, h != 0.0f ? log((double)S) - (double)a.in_entropy[r] : 0.0);
-    write_gradient<T>(a, r, x, token, M, LOG2E / temp, q, zero);
+    o.M = a.in_stats[2 * r];
+    o.c = LOG2E / temp;
+    o.q = RowGrad{0.0f, 0.0f, 0.0f};
+    o.zero = token < 0 || token >= a.V || (g == 0.0f && h == 0.0f) || S == 0.0f;
+    if (!o.zero) o.q = row_grad(g, h, temp, S, h != 0.0f ? log((double)S) - (double)a.in_entropy[r] : 0.0);
+    return o;
+}
+
+// Whether a row's logits are read at all.
+template <bool STATS> __device__ __forceinline__ bool row_read(const LossArgs &a, int r) {
+    if (STATS) {
+        const RowIn in = row_in(a, r);
+        return !in.idle && !in.status;
+    }
+    const int token = a.tokens[r];
+    return !(token < 0 || token >= a.V || (a.g_logprob[r] == 0.0f && !(a.g_entropy && a.g_entropy[r] != 0.0f)) || a.in_stats[2 * r + 1] == 0.0f);
+}
+
+// A warp's units of shared memory, filled in the order in which it will want them, row after row.
+template <class T, bool STATS, bool GRAD> struct Feed {
+    const LossArgs &a; const Layout &L;
+    uint4 *slots; uint64_t *bars;
+    int warp, warps;           // of the row's
+    int row0, step;            // this cluster's rows are row0, row0 + step, ...
+    int i, base; unsigned int mask;   // the row that is being fetched, and which of 32 rows are read
+    int u, pass;               // its next unit, and which time through the row
+    int ahead;                 // units fetched or on their way, not given back
+    int put, get, parity;      // slots
+    RowSpan<T> span;
+    bool more, late;
+    int owed, owed_slot, owed_parity;   // copies on their way when a wait ran out
+
+    __device__ __forceinline__ Feed(const LossArgs &a_, const Layout &L_, uint4 *s, uint64_t *b, int w, int ws, int r0, int st)
+        : a(a_), L(L_), slots(s), bars(b), warp(w), warps(ws), row0(r0), step(st), i(-1), base(-32), mask(0), u(0), pass(0), ahead(0), put(0), get(0), parity(0),
+          span((const T *)a_.logits, a_.V), more(true), late(false), owed(0) { next_row(); }
+    __device__ __forceinline__ bool row_ok(int k) const { return (long long)row0 + (long long)k * step < a.B; }
+    __device__ void next_row() {
+        for (;;) {
+            i++;
+            if (!row_ok(i)) { more = false; return; }
+            if (i - base >= 32) {
+                base = i;
+                const int lane = threadIdx.x & 31;
+                mask = __ballot_sync(0xffffffffu, row_ok(i + lane) && row_read<STATS>(a, row0 + (i + lane) * step));
+            }
+            if (!(mask >> (i - base) & 1)) continue;
+            span = RowSpan<T>((const T *)a.logits + (long long)(row0 + i * step) * a.row_stride, a.V);
+            u = warp; pass = 0;
+            if (u < span.units) return;
+        }
+    }
+    // as many units as there is room for
+    __device__ __forceinline__ void fetch() {
+        while (more && ahead < L.R) {
+            if ((threadIdx.x & 31) == 0) {
+                const int bytes = span.unit_bytes(u);
+                mbar_expect_tx(&bars[put], (uint32_t)bytes);
+                bulk_g2s(slots + (size_t)put * (UNIT * sizeof(T) / 16), span.x + (size_t)u * UNIT, (uint32_t)bytes, &bars[put]);
+            }
+            ahead++;
+            if (++put == L.R) put = 0;
+            u += warps;
+            if (u >= span.units) {
+                if (STATS && GRAD && !L.resident && pass == 0) { pass = 1; u = warp; }
+                else next_row();
+            }
+        }
+    }
+    __device__ __forceinline__ const uint4 *slot(int k) const { return slots + (size_t)k * (UNIT * sizeof(T) / 16); }
+    // the k-th unit from the oldest that has not been given back has arrived
+    __device__ __forceinline__ const uint4 *wait(int k) {
+        int s = get + k, p = parity;
+        if (s >= L.R) { s -= L.R; p ^= 1; }
+        if (!late) {
+            bool here = false;
+            for (int i = 0; i < WAIT_TRIES && !here; i++) here = mbar_try_wait(&bars[s], p);
+            if (__any_sync(0xffffffffu, !here)) { late = true; more = false; owed = ahead - k; owed_slot = s; owed_parity = p; }
+        }
+        return slot(s);
+    }
+    // before the block's shared memory goes back, what is on its way is waited for once more
+    __device__ void drain() {
+        for (; late && owed > 0; owed--) {
+            bool here = false;
+            for (int i = 0; i < WAIT_TRIES && !here; i++) here = mbar_try_wait(&bars[owed_slot], owed_parity);
+            if (++owed_slot == L.R) { owed_slot = 0; owed_parity ^= 1; }
+        }
+    }
+    __device__ __forceinline__ const uint4 *again(int k) const { int s = get + k; if (s >= L.R) s -= L.R; return slot(s); }
+    __device__ __forceinline__ void give_back() {
+        __syncwarp();
+        ahead--;
+        if (++get == L.R) { get = 0; parity ^= 1; }
+    }
+};
+
+// ---- the kernel ------------------------------------------------------------------------------------------
+//
+// STATS: a row's maximum and sums, logprob, entropy and loss. GRAD: its gradient, from those (the policy loss) or, without
+// STATS, from the ones of an earlier pass. ENT: entropies take part.
+//
+// A warp has a ring of shared memory to itself and fills it with bulk copies, units of 1024 logits that only it reads: nothing
+// waits for another warp but the row's sums. Where the row fits the rings of its cluster (resident) it is read from memory once: the units stay
+// until the gradient has been taken from them, and as they are given back the next row's come in, so reads and writes overlap.
+struct RowShare { float M, A, H, token; int zero; };
+
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void put_stat(Stat *st, const Stat &o, int C) {   // into every block of the cluster
+    const int lane = threadIdx.x & 31;
+    if (lane < C) {
+        uint32_t to;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(st)), "r"(lane));
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(o.m), "f"(o.s), "f"(o.w), "f"(__uint_as_float(o.late)) : "memory");
+    }
+}
+
+template <class T> size_t smem_of(const Layout &L) {
+    return (size_t)L.W * L.R * (UNIT * sizeof(T) + 8) + 2 * (size_t)(L.units + 1) * sizeof(Stat);
+}
+
+template <class T, bool STATS, bool GRAD, bool ENT>
+__global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_constant__ LossArgs a, const __grid_constant__ Layout L) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ RowShare share;
+    constexpr int UB = UNIT * sizeof(T), K = UB / 512;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, rank = blockIdx.x % L.C;
+    const int warp = rank * L.W + w, warps = L.C * L.W;
+    const int row0 = blockIdx.x / L.C, step = L.rows_at_once;
+    uint4 *slots = reinterpret_cast<uint4 *>(smem + (size_t)w * L.R * UB);
+    Stat *stats = reinterpret_cast<Stat *>(smem + (size_t)L.W * L.R * UB);   // [2][units + 1]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(stats + 2 * (L.units + 1)) + w * L.R;
+    if (STATS) cluster_begun();
+    for (int i = lane; i < L.R; i += 32) mbar_init(&bars[i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+    __syncwarp();
+    Feed<T, STATS, GRAD> feed(a, L, slots, bars, warp, warps, row0, step);
+    feed.fetch();
+    if (STATS) cluster_all_begun();
+    unsigned int mask = 0;
+    int side = 0;   // which of the two tables of stats: the other one may still be read
+    for (int i = 0; feed.row_ok(i); i++) {
+        const int r = row0 + i * step;
+        if (i % 32 == 0) mask = __ballot_sync(0xffffffffu, feed.row_ok(i + lane) && row_read<STATS>(a, row0 + (i + lane) * step));
+        T *out = GRAD ? (T *)a.grad + (long long)r * a.grad_stride : nullptr;
+        if (!(mask >> (i % 32) & 1)) {
+            if (STATS && warp == 0 && lane == 0) {
+                const RowIn in = row_in(a, r);
+                if (in.idle) row_idle(a, r); else row_answer(a, r, in, 0.0f, 0.0f, 1.0, 0.0, 1.0f, true);
+            }
+            if (GRAD) zero_row<T>(out, a.V, warp, warps);
+            continue;
+        }
+        const RowSpan<T> span((const T *)a.logits + (long long)r * a.row_stride, a.V);
+        const bool edge_mine = span.edge() && warp == span.units % warps;
+        const int edge_at = edge_mine ? span.edge_at(lane) : INT32_MIN;
+        const float edge = edge_at != INT32_MIN ? to_f32(span.x[edge_at]) : -INFINITY;
+        const int token = a.tokens[r];
+        float M, c, A, H, at_token;
+        bool zero = false;
+        if (STATS) {
+            const RowIn in = row_in(a, r);
+            c = LOG2E / in.T;
+            const float xt = w == 0 ? to_f32(span.x[token - span.head]) : 0.0f;
+            Stat *st = stats + side * (L.units + 1);
+            side ^= 1;
+            int n = 0;
+            for (int u = warp; u < span.units; u += warps) {
+                const uint4 *slot = feed.wait(n);
+                const int chunks = span.unit_bytes(u) >> 4;
+                uint4 v[K];
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    constexpr unsigned int low = Chunk<T>::LOWEST;
+                    v[k] = k * 32 + lane < chunks ? slot[k * 32 + lane] : make_uint4(low, low, low, low);
+                }
+                Stat o = unit_stat<T, ENT>(v, c);
+                o.late = feed.late || LOSS_KNOB(a, 16);   // (testing build: a wait that ran out)
+                put_stat(st + u, o, L.C);
+                if (GRAD && L.resident) n++;
+                else { feed.give_back(); feed.fetch(); }
+            }
+            if (edge_mine) put_stat(st + span.units, edge_stat<ENT>(edge, c), L.C);
+            cluster_sync();
+            if (w == 0) {
+                double S, W;
+                unsigned int late;
+                row_stat<ENT>(st, span.units + (span.edge() ? 1 : 0), c, M, S, W, late);
+                RowIn got = in;
+                if (late) got.status |= MOLLA_ROW_LOAD_TIMEOUT;
+                const RowGrad q = row_answer(a, r, got, xt, M, S, W, c, rank == 0 && lane == 0);
+                if (GRAD && lane == 0) share = RowShare{M, q.A, q.H, q.token, q.A == 0.0f && q.H == 0.0f && q.token == 0.0f};
+            }
+            if (!GRAD) continue;
+            __syncthreads();
+            M = share.M; A = share.A; H = share.H; at_token = share.token; zero = share.zero != 0;
+        } else {
+            const Given in = row_given(a, r);
+            M = in.M; c = in.c; A = in.q.A; H = in.q.H; at_token = in.q.token;
+        }
+        if (!GRAD) continue;
+        T *to = out + span.head;
+        const bool wide = ((uintptr_t)to & 15) == 0;
+        if (zero) zero_row<T>(out, a.V, warp, warps);
+        for (int u = warp; u < span.units; u += warps) {
+            const uint4 *slot = STATS && L.resident ? feed.again(0) : feed.wait(0);
+            if (!zero) {
+                const int bytes = span.unit_bytes(u);
+                unit_gradient<T, ENT>(slot, bytes, to + (size_t)u * UNIT, wide, M, c, feed.late ? NAN : A, H);
+                const int t = token - span.head - u * UNIT;
+                if (t >= 0 && t < bytes / (int)sizeof(T)) {
+                    __syncwarp();   // behind the store of the whole chunk
+                    if (lane == 0) to[(size_t)u * UNIT + t] = from_f32<T>(gradient_of<T, ENT>(to_f32(reinterpret_cast<const T *>(slot)[t]), M, c, A, H) + at_token);
+                }
+            }
+            feed.give_back();
+            feed.fetch();
+        }
+        if (edge_at != INT32_MIN && !zero)
+            to[edge_at] = from_f32<T>(gradient_of<T, ENT>(edge, M, c, A, H) + (edge_at == token - span.head ? at_token : 0.0f));
+    }
+    feed.drain();
+    if (STATS) cluster_sync();   // nobody leaves while another block writes its sums into this one
 }
 
 // ---- sums over rows ---------------------------------------------------------------------------------
@@ -292,24 +722,90 @@ __global__ void __launch_bounds__(ST) pairs_kernel(const __grid_constant__ PairA
     if (threadIdx.x == 0) *a.loss = (float)(total * (double)a.scale);
 }
 
-template <class K> cudaError_t launch_rows(K f32, K bf16, K fp16, const LossArgs &a, cudaStream_t st) {
+// ---- launches --------------------------------------------------------------------------------------------
+
+constexpr int MAX_DEVICES = 64;
+constexpr size_t BLOCK_SMEM_2 = 112 * 1024, BLOCK_SMEM_1 = 224 * 1024;   // dynamic shared memory of two blocks an SM, and of one
+
+int sm_count_of(int &dev) {
+    int sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { dev = -1; return 0; }
+    return sms;
+}
+
+template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms, int &blocks_per_sm) {
+    Layout L{};
+    const int UB = UNIT * (int)sizeof(T);
+    L.units = (V + UNIT - 1) / UNIT + 1;   // (an unaligned row's whole chunks, and its edge)
+    const int most = (V * (int)sizeof(T) + UB - 1) / UB;
+    const int room2 = (int)((BLOCK_SMEM_2 - 2 * (size_t)(L.units + 1) * sizeof(Stat)) / (UB + 8)), room1 = (int)((BLOCK_SMEM_1 - 2 * (size_t)(L.units + 1) * sizeof(Stat)) / (UB + 8));
+    int room = room2;
+    blocks_per_sm = 2;
+    L.C = 1;
+    if (STATS && GRAD) {
+        while (L.C < 8 && 4 * most > 3 * room2 * L.C) L.C *= 2;
+        if (most > room2 * L.C) { room = room1; blocks_per_sm = 1; }
+    }
+    while (L.C < 8 && (long long)B * L.C * 2 * 9 <= (long long)sms * blocks_per_sm * 8 && most > L.C * 8) L.C *= 2;
+    // as many warps as share the row's units most evenly
+    int best = 0x7fffffff;
+    for (int w = MAX_WARPS; w >= 6; w--) {
+        const int slots = (most + L.C * w - 1) / (L.C * w) * L.C * w;
+        if (slots < best) { best = slots; L.W = w; }
+    }
+    if (L.W > most) L.W = most > 0 ? most : 1;
+    const int each = (most + L.C * L.W - 1) / (L.C * L.W);
+    L.R = room / L.W;
+    if (L.R > 64) L.R = 64;
+    L.resident = each <= L.R;
+    return L;
+}
+
+template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(const LossArgs &a, cudaStream_t st) {
+    int dev = 0;
+    const int sms = sm_count_of(dev);
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    int per_sm = 1;
+    Layout L = layout_of<T, STATS, GRAD>(a.B, a.V, sms, per_sm);
+    const size_t smem = smem_of<T>(L);
+    auto kernel = rows_kernel<T, STATS, GRAD, ENT>;
+    static bool asked[MAX_DEVICES] = {};
+    if (dev >= MAX_DEVICES || !asked[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BLOCK_SMEM_1);
+        if (e != cudaSuccess) return e;
+        if (dev < MAX_DEVICES) asked[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    long long clusters = (long long)sms * per_sm / L.C;
+    if (clusters > a.B) clusters = a.B;
+    if (clusters < 1) clusters = 1;
+    L.rows_at_once = (int)clusters;
+    cfg.gridDim = dim3((unsigned int)(clusters * L.C)); cfg.blockDim = dim3(32u * (unsigned int)L.W); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned int)L.C; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = STATS && L.C > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, a, (const Layout)L);
+}
+
+template <bool STATS, bool GRAD> cudaError_t launch_type(const LossArgs &a, bool ent, cudaStream_t st) {
     if (a.B == 0) return cudaSuccess;
-    (a.type == MOLLA_LOGITS_FP32 ? f32 : a.type == MOLLA_LOGITS_BF16 ? bf16 : fp16)<<<a.B, NT, 0, st>>>(a);
-    return cudaGetLastError();
+    switch (a.type) {
+        case MOLLA_LOGITS_FP32: return ent ? launch_rows<float, STATS, GRAD, true>(a, st) : launch_rows<float, STATS, GRAD, false>(a, st);
+        case MOLLA_LOGITS_BF16: return ent ? launch_rows<__nv_bfloat16, STATS, GRAD, true>(a, st) : launch_rows<__nv_bfloat16, STATS, GRAD, false>(a, st);
+        default: return ent ? launch_rows<__half, STATS, GRAD, true>(a, st) : launch_rows<__half, STATS, GRAD, false>(a, st);
+    }
 }
 
 }  // namespace
 
-cudaError_t molla_loss_score(const LossArgs &a, cudaStream_t st) {
-    return launch_rows(rows_kernel<float>, rows_kernel<__nv_bfloat16>, rows_kernel<__half>, a, st);
-}
+cudaError_t molla_loss_score(const LossArgs &a, cudaStream_t st) { return launch_type<true, false>(a, a.entropy != nullptr, st); }
 
-cudaError_t molla_loss_backward(const LossArgs &a, cudaStream_t st) {
-    return launch_rows(backward_kernel<float>, backward_kernel<__nv_bfloat16>, backward_kernel<__half>, a, st);
-}
+cudaError_t molla_loss_backward(const LossArgs &a, cudaStream_t st) { return launch_type<false, true>(a, a.g_entropy != nullptr, st); }
 
 cudaError_t molla_loss_policy(const LossArgs &a, cudaStream_t st) {
-    const cudaError_t e = molla_loss_score(a, st);
+    const bool ent = a.entropy != nullptr || a.entropy_coef != 0.0f;
+    const cudaError_t e = a.grad ? launch_type<true, true>(a, ent, st) : launch_type<true, false>(a, ent, st);
     if (e != cudaSuccess) return e;
     row_sum_kernel<<<1, ST, 0, st>>>(a.row_loss, a.B, a.scale, a.loss);
     return cudaGetLastError();

@@ -18,6 +18,9 @@ struct LossArgs {
     const float *old_logprob; const float *advantage; const float *weight; const float *ref_logprob;
     float clip_low, clip_high, kl_coef, entropy_coef, scale, grad_scale;
     float *loss; float *row_loss; float *kl; unsigned char *clipped;
+#ifdef MOLLA_SAMPLE_TESTING
+    int knobs;                   // experiment switches (0 = production behaviour)
+#endif
 };
 
 // The preference loss between its two passes over the logits.

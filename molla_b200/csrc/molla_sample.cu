@@ -1821,6 +1821,9 @@ int loss_block(LossArgs &a, const void *logits, int type, int64_t row_stride, in
     if ((uintptr_t)logits % (type == MOLLA_LOGITS_FP32 ? 4 : 2)) return fail(MOLLA_ERR_ARGUMENT, "logits have to be aligned to their type%s");
     a.logits = logits; a.type = type; a.row_stride = row_stride; a.B = B; a.V = V;
     a.tokens = tokens; a.temperature = temperature;
+#ifdef MOLLA_SAMPLE_TESTING
+    a.knobs = g_knobs;
+#endif
     return MOLLA_OK;
 }
 

@@ -683,3 +683,31 @@ def test_a_rollout_from_sampling_to_both_losses(dev, lib):
     off = off[: len(off) - (len(off) + 1) % 2]
     check_preference(losses.preference_loss(later, tok, off, ref_logprob=ref, temperature=T),
                      preference_reference(later, tok, off, ref=ref, T=T))
+
+
+# ---- a load that never comes, as the testing build pretends ----------------------------------------------------------
+
+@pytest.mark.parametrize("V", [3000, 151936])
+def test_a_wait_that_runs_out_is_the_rows_status(dev, lib, V):
+    x, tok, gen = make(6, V, torch.bfloat16, dev)
+    old, ref, adv = rollout(x, tok, gen, dev)
+    off = torch.tensor([0, 3, 6], dtype=torch.int32, device=dev)
+    tok[2] = -1
+    with capi.testing_library() as T:
+        T.molla_sample_debug_knobs(16)
+        try:
+            a = losses.token_logprobs(x, tok, want_entropy=True)
+            b = losses.policy_loss(x, tok, old, adv)
+            c = losses.preference_loss(x, tok, off)
+        finally:
+            T.molla_sample_debug_knobs(0)
+        torch.cuda.synchronize()
+        late = [0 if r == 2 else capi.ROW_LOAD_TIMEOUT for r in range(6)]
+        for got in (a, b, c):
+            assert got["row_status"].tolist() == late
+            assert got["logprob"].isnan().tolist() == [r != 2 for r in range(6)]
+        assert bool(b["loss"].isnan()) and not b["grad_logits"].any()
+        assert c["pair_status"].tolist() == [capi.ROW_LOAD_TIMEOUT] and not c["grad_logits"].any()
+        assert not losses.token_logprobs_backward(x, tok, a, adv).any()
+        again = losses.token_logprobs(x, tok)
+    assert not again["row_status"].any() and bool(again["logprob"].isfinite().all())
