@@ -48,9 +48,10 @@ template <> __device__ __forceinline__ __half from_f32(float v) { return __float
 
 // ---- a row's scalars ------------------------------------------------------------------------------
 
+// A row's inputs; a lane fetches a row's, 32 rows ahead.
 struct RowIn {
     int token;
-    float T;             // temperature
+    float T, old, advantage, weight, ref, xt;   // temperature; the policy loss's; the token's logit
     unsigned int status; // why the row cannot be answered, before it is read
     bool idle;           // nothing to answer: no token, or no weight
 };
@@ -59,7 +60,9 @@ __device__ __forceinline__ RowIn row_in(const LossArgs &a, int r) {
     RowIn in;
     in.token = a.tokens[r];
     in.T = a.temperature ? a.temperature[r] : 1.0f;
-    in.idle = in.token == -1 || (a.weight && a.weight[r] == 0.0f);
+    in.weight = a.weight ? a.weight[r] : 1.0f;
+    in.old = in.advantage = in.ref = in.xt = 0.0f;
+    in.idle = in.token == -1 || in.weight == 0.0f;
     in.status = 0;
     if (!in.idle) {
         if (in.token < 0 || in.token >= a.V) in.status |= MOLLA_ROW_BAD_TOKEN;
@@ -72,43 +75,61 @@ __device__ __forceinline__ RowIn row_in(const LossArgs &a, int r) {
 // The gradient's three numbers: add at the token, and A and H of the formula.
 struct RowGrad { float token, A, H; };
 
-__device__ __forceinline__ RowGrad row_grad(double g, double h, float T, double S, double w_over_st) {
+__device__ __forceinline__ RowGrad row_grad(float g, float h, float T, float S, float w_over_st) {
     RowGrad o;
-    const double inv = 1.0 / ((double)T * S);
-    o.token = (float)(g / (double)T);
-    o.A = (float)((g - h * w_over_st) * inv);
-    o.H = (float)(h * inv / (double)T);
+    const float inv = 1.0f / (T * S);
+    o.token = g / T;
+    o.A = (g - h * w_over_st) * inv;
+    o.H = h * inv / T;
     return o;
 }
 
-// What a row answers once its maximum M, sum S and, where entropies are wanted, W are known. One thread.
-__device__ RowGrad row_answer(const LossArgs &a, int r, const RowIn &in, float xt, float M, double S, double W, float c, bool write) {
+// ln S, S > 0: the power of two apart, the rest (within a factor of the square root of two of one) is below 0.35 and good to 3e-8
+// in 32 bits. (With log, exp and the divisions in 64 bits a row's scalars took 6200 cycles, in which its blocks wait.)
+__device__ __forceinline__ double ln_of(double S) {
+    if (!(S > 0.0) || isinf(S)) return S == 0.0 ? -INFINITY : S;   // (NaN stays)
+    int k = __double2hiint(S) - 0x3fe6a09e;   // the exponent of S / sqrt(1/2)
+    k >>= 20;
+    const double f = __hiloint2double(__double2hiint(S) - (k << 20), __double2loint(S));
+    return (double)k * 0.693147180559945309 + (double)log1pf((float)(f - 1.0));
+}
+
+// exp(q) - 1 - q: for small q from its series, which the difference would lose
+__device__ __forceinline__ float exp_less_line(float q) {
+    if (fabsf(q) > 0.5f) return __fsub_rn(expm1f(q), q);
+    float p = 1.0f / 3628800.0f;
+    p = __fmaf_rn(p, q, 1.0f / 362880.0f); p = __fmaf_rn(p, q, 1.0f / 40320.0f); p = __fmaf_rn(p, q, 1.0f / 5040.0f);
+    p = __fmaf_rn(p, q, 1.0f / 720.0f); p = __fmaf_rn(p, q, 1.0f / 120.0f); p = __fmaf_rn(p, q, 1.0f / 24.0f);
+    p = __fmaf_rn(p, q, 1.0f / 6.0f); p = __fmaf_rn(p, q, 0.5f);
+    return p * q * q;
+}
+
+// What a row answers once its maximum M, sum S and, where entropies are wanted, W are known.
+__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, int r, const RowIn &in, float M, double S, double W, float c, bool write) {
     const unsigned int status = in.status | (M == -INFINITY && S == 0.0 && !in.status ? MOLLA_ROW_EMPTY : 0u);
     // ln p in the temperature that c stands for (log2(e)/T rounded): the error of c then moves ln S and the token together
-    const double T = LOG2E_64 / (double)c, lnS = log(S);
-    const double l = ((double)xt - (double)M) / T - lnS;
-    const bool want_entropy = a.entropy != nullptr || a.entropy_coef != 0.0f;
-    const double w_over_st = want_entropy ? W / (S * T) : 0.0;
-    const double H = lnS - w_over_st;
-    RowGrad o{0.0f, 0.0f, 0.0f};
+    const double to_nats = (double)c * 0.693147180559945309, lnS = ln_of(S);
+    const double l = ((double)in.xt - (double)M) * to_nats - lnS;
+    const float mean = (float)W / (float)S * (float)to_nats;   // of (x - M)/T
+    const double H = lnS - (double)mean;
     if (write) {
         a.status[r] = status;
         a.logprob[r] = status ? NAN : (float)l;
         if (a.entropy) a.entropy[r] = status ? NAN : (float)H;
         if (a.stats) { a.stats[2 * r] = status ? NAN : M; a.stats[2 * r + 1] = status ? 0.0f : (float)S; }
     }
-    if (!a.row_loss) return o;
+    if (!a.row_loss) return RowGrad{0.0f, 0.0f, 0.0f};
     // the policy loss
-    const double w = a.weight ? (double)a.weight[r] : 1.0;
-    const double ratio = exp(l - (double)a.old_logprob[r]), adv = a.advantage[r];
+    const double w = in.weight, adv = in.advantage;
+    const double ratio = expf((float)(l - (double)in.old));
     const double lo = 1.0 - (double)a.clip_low, hi = 1.0 + (double)a.clip_high;
     const double u = ratio * adv, v = fmin(fmax(ratio, lo), hi) * adv;
     const bool held = v < u;
     double term = -(held ? v : u), g = held ? 0.0 : -u;   // (a ratio that is NaN is not held)
     if (a.ref_logprob) {
-        const double q = (double)a.ref_logprob[r] - l, eq = expm1(q), kl = eq - q;
-        if (a.kl && write) a.kl[r] = status ? NAN : (float)kl;
-        if (a.kl_coef != 0.0f) { term += (double)a.kl_coef * kl; g -= (double)a.kl_coef * eq; }
+        const float q = (float)((double)in.ref - l), kl = exp_less_line(q);
+        if (a.kl && write) a.kl[r] = status ? NAN : kl;
+        if (a.kl_coef != 0.0f) { term += (double)a.kl_coef * (double)kl; g -= (double)a.kl_coef * ((double)kl + (double)q); }
     }
     double h = 0.0;
     if (a.entropy_coef != 0.0f) { term -= (double)a.entropy_coef * H; h = -w * (double)a.entropy_coef; }
@@ -117,8 +138,7 @@ __device__ RowGrad row_answer(const LossArgs &a, int r, const RowIn &in, float x
         if (a.clipped) a.clipped[r] = !status && held;
     }
     const double gs = (double)a.scale * (double)a.grad_scale;
-    if (!status) o = row_grad(g * w * gs, h * gs, in.T, S, w_over_st);
-    return o;
+    return status ? RowGrad{0.0f, 0.0f, 0.0f} : row_grad((float)(g * w * gs), (float)(h * gs), in.T, (float)S, mean);
 }
 
 __device__ void row_idle(const LossArgs &a, int r) {
@@ -208,7 +228,7 @@ template <> struct Chunk<__half> {
 // ---- rows by clusters, a unit of 1024 logits by a warp ------------------------------------------------
 
 constexpr int UNIT = 1024;
-constexpr int MAX_WARPS = 16;
+constexpr int MAX_WARPS = 16;      // with the one that answers
 constexpr int WAIT_TRIES = 1 << 22;   // of a bounded wait
 
 // How a launch lays its rows out: C blocks of W warps a row, R units of shared memory a warp, `rows_at_once` rows
@@ -400,17 +420,16 @@ template <class T> __device__ void zero_row(T *out, int V, int warp, int warps) 
 }
 
 // What a row's gradient is made of, where it is given (the backward pass).
-struct Given { bool zero; float M, c; RowGrad q; };
-__device__ __forceinline__ Given row_given(const LossArgs &a, int r) {
-    Given o;
-    const int token = a.tokens[r];
-    const float temp = a.temperature ? a.temperature[r] : 1.0f, S = a.in_stats[2 * r + 1];
+struct RowShare { float M, c, A, H, token_add; int token; int zero, pad; };
+__device__ __forceinline__ RowShare row_given(const LossArgs &a, int r) {
+    RowShare o = {};
+    const float T = a.temperature ? a.temperature[r] : 1.0f, S = a.in_stats[2 * r + 1];
     const float g = a.g_logprob[r], h = a.g_entropy ? a.g_entropy[r] : 0.0f;
+    o.token = a.tokens[r];
     o.M = a.in_stats[2 * r];
-    o.c = LOG2E / temp;
-    o.q = RowGrad{0.0f, 0.0f, 0.0f};
-    o.zero = token < 0 || token >= a.V || (g == 0.0f && h == 0.0f) || S == 0.0f;
-    if (!o.zero) o.q = row_grad(g, h, temp, S, h != 0.0f ? log((double)S) - (double)a.in_entropy[r] : 0.0);
+    o.c = LOG2E / T;
+    const RowGrad q = row_grad(g, h, T, S, h != 0.0f ? (float)(ln_of(S) - (double)a.in_entropy[r]) : 0.0f);
+    o.A = q.A; o.H = q.H; o.token_add = q.token;
     return o;
 }
 
@@ -482,9 +501,15 @@ template <class T, bool STATS, bool GRAD> struct Feed {
         if (!late) {
             bool here = false;
             for (int i = 0; i < WAIT_TRIES && !here; i++) here = mbar_try_wait(&bars[s], p);
-            if (__any_sync(0xffffffffu, !here)) { late = true; more = false; owed = ahead - k; owed_slot = s; owed_parity = p; }
+            if (__any_sync(0xffffffffu, !here)) lose(k);
         }
         return slot(s);
+    }
+    // a wait ran out, with the units from the k-th on still on their way: nothing more is waited for or fetched
+    __device__ void lose(int k = 0) {
+        late = true; more = false;
+        owed = ahead - k; owed_slot = get + k; owed_parity = parity;
+        if (owed_slot >= L.R) { owed_slot -= L.R; owed_parity ^= 1; }
     }
     // before the block's shared memory goes back, what is on its way is waited for once more
     __device__ void drain() {
@@ -510,56 +535,151 @@ template <class T, bool STATS, bool GRAD> struct Feed {
 // A warp has a ring of shared memory to itself and fills it with bulk copies, units of 1024 logits that only it reads: nothing
 // waits for another warp but the row's sums. Where the row fits the rings of its cluster (resident) it is read from memory once: the units stay
 // until the gradient has been taken from them, and as they are given back the next row's come in, so reads and writes overlap.
-struct RowShare { float M, A, H, token; int zero; };
+//
+// The sums of all units go to the cluster's first block, where one warp does nothing but put them together, answer for the row and
+// tell the gradient's numbers to all blocks; it has fetched the rows' inputs beforehand. (As a part of one of the
+// ordinary warps' work, between two barriers, that took 12 of 29 thousand cycles a row.)
+constexpr int DEPTH = 4;   // rows whose sums may be on their way
+
+struct Control {
+    RowShare share[DEPTH];
+    uint64_t sums[DEPTH];      // all warps' sums of a row are there (used in the cluster's first block)
+    uint64_t answered[DEPTH];  // ... and have been read, and `share` has what they came to
+};
 
 __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-
-__device__ __forceinline__ void put_stat(Stat *st, const Stat &o, int C) {   // into every block of the cluster
-    const int lane = threadIdx.x & 31;
-    if (lane < C) {
-        uint32_t to;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(st)), "r"(lane));
-        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(o.m), "f"(o.s), "f"(o.w), "f"(__uint_as_float(o.late)) : "memory");
+__device__ __forceinline__ uint32_t at_rank(const void *p, int rank) {
+    uint32_t to;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(p)), "r"(rank));
+    return to;
+}
+__device__ __forceinline__ void put16(uint32_t to, float x, float y, float z, float w) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// whether a phase of a barrier that other blocks arrive at has ended (all lanes alike)
+__device__ __forceinline__ bool wait_cluster(uint64_t *bar, int parity) {
+    bool here = false;
+    for (int i = 0; i < WAIT_TRIES && !here; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        here = ok != 0;
     }
+    return __all_sync(0xffffffffu, here);
 }
 
 template <class T> size_t smem_of(const Layout &L) {
-    return (size_t)L.W * L.R * (UNIT * sizeof(T) + 8) + 2 * (size_t)(L.units + 1) * sizeof(Stat);
+    return (size_t)L.W * L.R * (UNIT * sizeof(T) + 8) + DEPTH * (size_t)(L.units + 1) * sizeof(Stat);
+}
+
+// The warp that answers for the rows of a cluster.
+template <class T, bool GRAD, bool ENT>
+__device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, Control &ctl, const Stat *stats, int row0, int step) {
+    const int lane = threadIdx.x & 31;
+    bool late = false;
+    int n = 0;   // rows that are read
+    RowIn mine = {};
+    unsigned int mask = 0;
+    for (int i = 0; (long long)row0 + (long long)i * step < a.B; i++) {
+        if (i % 32 == 0) {
+            const long long r = (long long)row0 + (long long)(i + lane) * step;
+            bool read = false;
+            if (r < a.B) {
+                mine = row_in(a, (int)r);
+                read = !mine.idle && !mine.status;
+                if (read) mine.xt = to_f32(((const T *)a.logits)[r * a.row_stride + mine.token]);
+                if (a.row_loss) {
+                    mine.old = a.old_logprob[r]; mine.advantage = a.advantage[r];
+                    if (a.ref_logprob) mine.ref = a.ref_logprob[r];
+                }
+                if (mine.idle) row_idle(a, (int)r);
+                else if (mine.status) row_answer(a, (int)r, mine, 0.0f, 1.0, 0.0, 1.0f, true);
+            }
+            mask = __ballot_sync(0xffffffffu, read);
+        }
+        if (!(mask >> (i % 32) & 1)) continue;
+        const int r = row0 + i * step, from = i % 32, s = n % DEPTH;
+        RowIn in;
+        in.token = __shfl_sync(0xffffffffu, mine.token, from); in.T = __shfl_sync(0xffffffffu, mine.T, from);
+        in.old = __shfl_sync(0xffffffffu, mine.old, from); in.advantage = __shfl_sync(0xffffffffu, mine.advantage, from);
+        in.weight = __shfl_sync(0xffffffffu, mine.weight, from); in.ref = __shfl_sync(0xffffffffu, mine.ref, from);
+        in.xt = __shfl_sync(0xffffffffu, mine.xt, from);
+        in.status = 0; in.idle = false;
+        const RowSpan<T> span((const T *)a.logits + (long long)r * a.row_stride, a.V);
+        const float c = LOG2E / in.T;
+        if (!late) late = !wait_cluster(&ctl.sums[s], (n / DEPTH) & 1);
+        float M;
+        double S, W;
+        unsigned int missed;
+        row_stat<ENT>(stats + s * (L.units + 1), span.units + (span.edge() ? 1 : 0), c, M, S, W, missed);
+        late = late || missed;   // (what was lost once has the barriers out of step)
+        if (late) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
+        const RowGrad q = row_answer(a, r, in, M, S, W, c, lane == 0);
+        __syncwarp();
+        if (lane < L.C) {
+            if (GRAD) {
+                const uint32_t to = at_rank(&ctl.share[s], lane);
+                put16(to, M, c, q.A, q.H);
+                put16(to + 16, q.token, __int_as_float(in.token), __int_as_float(q.A == 0.0f && q.H == 0.0f && q.token == 0.0f), 0.0f);
+            }
+            arrive(at_rank(&ctl.answered[s], lane));
+        }
+        n++;
+    }
 }
 
 template <class T, bool STATS, bool GRAD, bool ENT>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_constant__ LossArgs a, const __grid_constant__ Layout L) {
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ RowShare share;
+    __shared__ Control ctl;
     constexpr int UB = UNIT * sizeof(T), K = UB / 512;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, rank = blockIdx.x % L.C;
     const int warp = rank * L.W + w, warps = L.C * L.W;
     const int row0 = blockIdx.x / L.C, step = L.rows_at_once;
     uint4 *slots = reinterpret_cast<uint4 *>(smem + (size_t)w * L.R * UB);
-    Stat *stats = reinterpret_cast<Stat *>(smem + (size_t)L.W * L.R * UB);   // [2][units + 1]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(stats + 2 * (L.units + 1)) + w * L.R;
-    if (STATS) cluster_begun();
-    for (int i = lane; i < L.R; i += 32) mbar_init(&bars[i], 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    Stat *stats = reinterpret_cast<Stat *>(smem + (size_t)L.W * L.R * UB);   // [DEPTH][units + 1]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(stats + DEPTH * (L.units + 1)) + w * L.R;
+    if (STATS) {
+        if (threadIdx.x < DEPTH) {
+            mbar_init(&ctl.sums[threadIdx.x], warps);
+            mbar_init(&ctl.answered[threadIdx.x], 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (w < L.W)
+        for (int i = lane; i < L.R; i += 32) mbar_init(&bars[i], 1);
     fence_proxy_async();
-    __syncwarp();
+    if (STATS) cluster_sync();
+    else __syncwarp();
+    if (STATS && w == L.W) {
+        if (rank == 0) answer_rows<T, GRAD, ENT>(a, L, ctl, stats, row0, step);
+        cluster_sync();
+        return;
+    }
     Feed<T, STATS, GRAD> feed(a, L, slots, bars, warp, warps, row0, step);
     feed.fetch();
-    if (STATS) cluster_all_begun();
     unsigned int mask = 0;
-    int side = 0;   // which of the two tables of stats: the other one may still be read
+    RowShare mine = {};   // a row a lane: without STATS all of it, else c
+    int n = 0;            // rows that are read
     for (int i = 0; feed.row_ok(i); i++) {
-        const int r = row0 + i * step;
-        if (i % 32 == 0) mask = __ballot_sync(0xffffffffu, feed.row_ok(i + lane) && row_read<STATS>(a, row0 + (i + lane) * step));
+        const int r = row0 + i * step, from = i % 32;
+        if (from == 0) {
+            const bool ok = feed.row_ok(i + lane), read = ok && row_read<STATS>(a, row0 + (i + lane) * step);
+            mask = __ballot_sync(0xffffffffu, read);
+            if (!STATS && read) mine = row_given(a, row0 + (i + lane) * step);
+            if (STATS) mine.c = LOG2E / (read && a.temperature ? a.temperature[row0 + (i + lane) * step] : 1.0f);
+        }
         T *out = GRAD ? (T *)a.grad + (long long)r * a.grad_stride : nullptr;
-        if (!(mask >> (i % 32) & 1)) {
-            if (STATS && warp == 0 && lane == 0) {
-                const RowIn in = row_in(a, r);
-                if (in.idle) row_idle(a, r); else row_answer(a, r, in, 0.0f, 0.0f, 1.0, 0.0, 1.0f, true);
-            }
+        if (!(mask >> from & 1)) {
             if (GRAD) zero_row<T>(out, a.V, warp, warps);
             continue;
         }
@@ -567,72 +687,66 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         const bool edge_mine = span.edge() && warp == span.units % warps;
         const int edge_at = edge_mine ? span.edge_at(lane) : INT32_MIN;
         const float edge = edge_at != INT32_MIN ? to_f32(span.x[edge_at]) : -INFINITY;
-        const int token = a.tokens[r];
-        float M, c, A, H, at_token;
-        bool zero = false;
+        RowShare q;
+        q.c = __shfl_sync(0xffffffffu, mine.c, from);
         if (STATS) {
-            const RowIn in = row_in(a, r);
-            c = LOG2E / in.T;
-            const float xt = w == 0 ? to_f32(span.x[token - span.head]) : 0.0f;
-            Stat *st = stats + side * (L.units + 1);
-            side ^= 1;
-            int n = 0;
+            const int s = n % DEPTH;
+            // without a gradient nobody waits for a row's answer: its table has to be free again
+            if (!GRAD && n >= DEPTH && !feed.late && !wait_cluster(&ctl.answered[s], (n / DEPTH + 1) & 1)) feed.lose();
+            const uint32_t st = at_rank(stats + s * (L.units + 1), 0);
+            int k = 0;
             for (int u = warp; u < span.units; u += warps) {
-                const uint4 *slot = feed.wait(n);
+                const uint4 *slot = feed.wait(k);
                 const int chunks = span.unit_bytes(u) >> 4;
                 uint4 v[K];
 #pragma unroll
-                for (int k = 0; k < K; k++) {
+                for (int j = 0; j < K; j++) {
                     constexpr unsigned int low = Chunk<T>::LOWEST;
-                    v[k] = k * 32 + lane < chunks ? slot[k * 32 + lane] : make_uint4(low, low, low, low);
+                    v[j] = j * 32 + lane < chunks ? slot[j * 32 + lane] : make_uint4(low, low, low, low);
                 }
-                Stat o = unit_stat<T, ENT>(v, c);
+                Stat o = unit_stat<T, ENT>(v, q.c);
                 o.late = feed.late || LOSS_KNOB(a, 16);   // (testing build: a wait that ran out)
-                put_stat(st + u, o, L.C);
-                if (GRAD && L.resident) n++;
+                if (lane == 0) put16(st + u * (uint32_t)sizeof(Stat), o.m, o.s, o.w, __uint_as_float(o.late));
+                if (GRAD && L.resident) k++;
                 else { feed.give_back(); feed.fetch(); }
             }
-            if (edge_mine) put_stat(st + span.units, edge_stat<ENT>(edge, c), L.C);
-            cluster_sync();
-            if (w == 0) {
-                double S, W;
-                unsigned int late;
-                row_stat<ENT>(st, span.units + (span.edge() ? 1 : 0), c, M, S, W, late);
-                RowIn got = in;
-                if (late) got.status |= MOLLA_ROW_LOAD_TIMEOUT;
-                const RowGrad q = row_answer(a, r, got, xt, M, S, W, c, rank == 0 && lane == 0);
-                if (GRAD && lane == 0) share = RowShare{M, q.A, q.H, q.token, q.A == 0.0f && q.H == 0.0f && q.token == 0.0f};
+            if (edge_mine) {
+                const Stat o = edge_stat<ENT>(edge, q.c);
+                if (lane == 0) put16(st + span.units * (uint32_t)sizeof(Stat), o.m, o.s, o.w, 0.0f);
             }
+            if (lane == 0) arrive(at_rank(&ctl.sums[s], 0));
+            n++;
             if (!GRAD) continue;
-            __syncthreads();
-            M = share.M; A = share.A; H = share.H; at_token = share.token; zero = share.zero != 0;
+            if (!feed.late && !wait_cluster(&ctl.answered[s], ((n - 1) / DEPTH) & 1)) feed.lose();
+            q = ctl.share[s];
         } else {
-            const Given in = row_given(a, r);
-            M = in.M; c = in.c; A = in.q.A; H = in.q.H; at_token = in.q.token;
+            q.M = __shfl_sync(0xffffffffu, mine.M, from); q.A = __shfl_sync(0xffffffffu, mine.A, from); q.H = __shfl_sync(0xffffffffu, mine.H, from);
+            q.token_add = __shfl_sync(0xffffffffu, mine.token_add, from); q.token = __shfl_sync(0xffffffffu, mine.token, from);
+            q.zero = 0;
         }
         if (!GRAD) continue;
         T *to = out + span.head;
         const bool wide = ((uintptr_t)to & 15) == 0;
-        if (zero) zero_row<T>(out, a.V, warp, warps);
+        if (q.zero) zero_row<T>(out, a.V, warp, warps);
         for (int u = warp; u < span.units; u += warps) {
             const uint4 *slot = STATS && L.resident ? feed.again(0) : feed.wait(0);
-            if (!zero) {
+            if (!q.zero) {
                 const int bytes = span.unit_bytes(u);
-                unit_gradient<T, ENT>(slot, bytes, to + (size_t)u * UNIT, wide, M, c, feed.late ? NAN : A, H);
-                const int t = token - span.head - u * UNIT;
+                unit_gradient<T, ENT>(slot, bytes, to + (size_t)u * UNIT, wide, q.M, q.c, feed.late ? NAN : q.A, q.H);
+                const int t = q.token - span.head - u * UNIT;
                 if (t >= 0 && t < bytes / (int)sizeof(T)) {
                     __syncwarp();   // behind the store of the whole chunk
-                    if (lane == 0) to[(size_t)u * UNIT + t] = from_f32<T>(gradient_of<T, ENT>(to_f32(reinterpret_cast<const T *>(slot)[t]), M, c, A, H) + at_token);
+                    if (lane == 0) to[(size_t)u * UNIT + t] = from_f32<T>(gradient_of<T, ENT>(to_f32(reinterpret_cast<const T *>(slot)[t]), q.M, q.c, q.A, q.H) + q.token_add);
                 }
             }
             feed.give_back();
             feed.fetch();
         }
-        if (edge_at != INT32_MIN && !zero)
-            to[edge_at] = from_f32<T>(gradient_of<T, ENT>(edge, M, c, A, H) + (edge_at == token - span.head ? at_token : 0.0f));
+        if (edge_at != INT32_MIN && !q.zero)
+            to[edge_at] = from_f32<T>(gradient_of<T, ENT>(edge, q.M, q.c, q.A, q.H) + (edge_at == q.token - span.head ? q.token_add : 0.0f));
     }
     feed.drain();
-    if (STATS) cluster_sync();   // nobody leaves while another block writes its sums into this one
+    if (STATS) cluster_sync();   // nobody leaves while another block has something for it
 }
 
 // ---- sums over rows ---------------------------------------------------------------------------------
@@ -738,7 +852,7 @@ template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms
     const int UB = UNIT * (int)sizeof(T);
     L.units = (V + UNIT - 1) / UNIT + 1;   // (an unaligned row's whole chunks, and its edge)
     const int most = (V * (int)sizeof(T) + UB - 1) / UB;
-    const int room2 = (int)((BLOCK_SMEM_2 - 2 * (size_t)(L.units + 1) * sizeof(Stat)) / (UB + 8)), room1 = (int)((BLOCK_SMEM_1 - 2 * (size_t)(L.units + 1) * sizeof(Stat)) / (UB + 8));
+    const int room2 = (int)((BLOCK_SMEM_2 - DEPTH * (size_t)(L.units + 1) * sizeof(Stat)) / (UB + 8)), room1 = (int)((BLOCK_SMEM_1 - DEPTH * (size_t)(L.units + 1) * sizeof(Stat)) / (UB + 8));
     int room = room2;
     blocks_per_sm = 2;
     L.C = 1;
@@ -749,7 +863,7 @@ template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms
     while (L.C < 8 && (long long)B * L.C * 2 * 9 <= (long long)sms * blocks_per_sm * 8 && most > L.C * 8) L.C *= 2;
     // as many warps as share the row's units most evenly
     int best = 0x7fffffff;
-    for (int w = MAX_WARPS; w >= 6; w--) {
+    for (int w = STATS ? MAX_WARPS - 1 : MAX_WARPS; w >= 6; w--) {
         const int slots = (most + L.C * w - 1) / (L.C * w) * L.C * w;
         if (slots < best) { best = slots; L.W = w; }
     }
@@ -781,7 +895,7 @@ template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(cons
     if (clusters > a.B) clusters = a.B;
     if (clusters < 1) clusters = 1;
     L.rows_at_once = (int)clusters;
-    cfg.gridDim = dim3((unsigned int)(clusters * L.C)); cfg.blockDim = dim3(32u * (unsigned int)L.W); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.gridDim = dim3((unsigned int)(clusters * L.C)); cfg.blockDim = dim3(32u * (unsigned int)(L.W + (STATS ? 1 : 0))); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned int)L.C; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = STATS && L.C > 1 ? 1 : 0;
