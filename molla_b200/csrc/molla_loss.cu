@@ -105,12 +105,12 @@ __device__ __forceinline__ float exp_less_line(float q) {
 }
 
 // What a row answers once its maximum M, sum S and, where entropies are wanted, W are known.
-__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, int r, const RowIn &in, float M, double S, double W, float c, bool write) {
+__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, int r, const RowIn &in, float M, double S, float W, float c, bool write) {
     const unsigned int status = in.status | (M == -INFINITY && S == 0.0 && !in.status ? MOLLA_ROW_EMPTY : 0u);
     // ln p in the temperature that c stands for (log2(e)/T rounded): the error of c then moves ln S and the token together
     const double to_nats = (double)c * 0.693147180559945309, lnS = ln_of(S);
     const double l = ((double)in.xt - (double)M) * to_nats - lnS;
-    const float mean = (float)W / (float)S * (float)to_nats;   // of (x - M)/T
+    const float mean = W / (float)S * (float)to_nats;   // of (x - M)/T
     const double H = lnS - (double)mean;
     if (write) {
         a.status[r] = status;
@@ -151,90 +151,74 @@ __device__ void row_idle(const LossArgs &a, int r) {
     if (a.clipped) a.clipped[r] = 0;
 }
 
-// ---- packed pairs, and a 16-byte chunk of logits -----------------------------------------------------
+// ---- a 16-byte chunk of logits -----------------------------------------------------------------------
+// (Sums of pairs in packed 64-bit registers were tried: half of the additions, and three moves an element to pack them.)
 
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float lo, float hi) { f32x2 v; asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); return v; }
-__device__ __forceinline__ void unpack2(f32x2 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 v; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b)); return v; }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 v; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b)); return v; }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 v; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c)); return v; }
+__device__ __forceinline__ unsigned int word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ void set_word(uint4 &v, int i, unsigned int w) { if (i == 0) v.x = w; else if (i == 1) v.y = w; else if (i == 2) v.z = w; else v.w = w; }
+template <class V> __device__ __forceinline__ V as(unsigned int w) { return *reinterpret_cast<const V *>(&w); }
+template <class V> __device__ __forceinline__ unsigned int bits(const V &v) { return *reinterpret_cast<const unsigned int *>(&v); }
 
+// max: the larger of words of two chunks; top: the largest of a word; get and put: an element
 template <class T> struct Chunk;
 template <> struct Chunk<float> {
     static constexpr int N = 4;
-    __device__ static __forceinline__ f32x2 pair(const uint4 &v, int i) {
-        return i == 0 ? pack2(__uint_as_float(v.x), __uint_as_float(v.y)) : pack2(__uint_as_float(v.z), __uint_as_float(v.w));
+    __device__ static __forceinline__ unsigned int max(unsigned int a, unsigned int b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+    __device__ static __forceinline__ float top(unsigned int w) { return __uint_as_float(w); }
+    __device__ static __forceinline__ void get(const uint4 &v, float (&x)[N]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = __uint_as_float(word(v, i));
     }
-    __device__ static __forceinline__ float most(const uint4 &v) {
-        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
-    }
-    __device__ static __forceinline__ uint4 most2(const uint4 &a, const uint4 &b) {
-        return make_uint4(m(a.x, b.x), m(a.y, b.y), m(a.z, b.z), m(a.w, b.w));
-    }
-    __device__ static __forceinline__ unsigned int m(unsigned int a, unsigned int b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
-    __device__ static __forceinline__ void put(uint4 &o, int i, float lo, float hi) {
-        if (i == 0) { o.x = __float_as_uint(lo); o.y = __float_as_uint(hi); } else { o.z = __float_as_uint(lo); o.w = __float_as_uint(hi); }
+    __device__ static __forceinline__ uint4 put(const float (&x)[N]) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
     }
     static constexpr unsigned int LOWEST = 0xff800000u;   // -inf
 };
-__device__ __forceinline__ unsigned int word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-__device__ __forceinline__ void set_word(uint4 &v, int i, unsigned int w) { if (i == 0) v.x = w; else if (i == 1) v.y = w; else if (i == 2) v.z = w; else v.w = w; }
 template <> struct Chunk<__nv_bfloat16> {
     static constexpr int N = 8;
-    __device__ static __forceinline__ f32x2 pair(const uint4 &v, int i) {
-        const unsigned int w = word(v, i);
-        return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    __device__ static __forceinline__ unsigned int max(unsigned int a, unsigned int b) { return bits(__hmax2(as<__nv_bfloat162>(a), as<__nv_bfloat162>(b))); }
+    __device__ static __forceinline__ float top(unsigned int w) { return fmaxf(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    __device__ static __forceinline__ void get(const uint4 &v, float (&x)[N]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) { const unsigned int w = word(v, i); x[2 * i] = __uint_as_float(w << 16); x[2 * i + 1] = __uint_as_float(w & 0xffff0000u); }
     }
-    __device__ static __forceinline__ unsigned int m(unsigned int a, unsigned int b) {
-        const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-        return *reinterpret_cast<const unsigned int *>(&r);
-    }
-    __device__ static __forceinline__ uint4 most2(const uint4 &a, const uint4 &b) { return make_uint4(m(a.x, b.x), m(a.y, b.y), m(a.z, b.z), m(a.w, b.w)); }
-    __device__ static __forceinline__ float most(const uint4 &v) {
-        const unsigned int w = m(m(v.x, v.y), m(v.z, v.w));
-        return fmaxf(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-    }
-    __device__ static __forceinline__ void put(uint4 &o, int i, float lo, float hi) {
-        const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
-        set_word(o, i, *reinterpret_cast<const unsigned int *>(&r));
+    __device__ static __forceinline__ uint4 put(const float (&x)[N]) {
+        uint4 o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) set_word(o, i, bits(__floats2bfloat162_rn(x[2 * i], x[2 * i + 1])));
+        return o;
     }
     static constexpr unsigned int LOWEST = 0xff80ff80u;
 };
 template <> struct Chunk<__half> {
     static constexpr int N = 8;
-    __device__ static __forceinline__ f32x2 pair(const uint4 &v, int i) {
-        const unsigned int w = word(v, i);
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-        return pack2(f.x, f.y);
+    __device__ static __forceinline__ unsigned int max(unsigned int a, unsigned int b) { return bits(__hmax2(as<__half2>(a), as<__half2>(b))); }
+    __device__ static __forceinline__ float top(unsigned int w) { const float2 f = __half22float2(as<__half2>(w)); return fmaxf(f.x, f.y); }
+    __device__ static __forceinline__ void get(const uint4 &v, float (&x)[N]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) { const float2 f = __half22float2(as<__half2>(word(v, i))); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
     }
-    __device__ static __forceinline__ unsigned int m(unsigned int a, unsigned int b) {
-        const __half2 r = __hmax2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
-        return *reinterpret_cast<const unsigned int *>(&r);
-    }
-    __device__ static __forceinline__ uint4 most2(const uint4 &a, const uint4 &b) { return make_uint4(m(a.x, b.x), m(a.y, b.y), m(a.z, b.z), m(a.w, b.w)); }
-    __device__ static __forceinline__ float most(const uint4 &v) {
-        const unsigned int w = m(m(v.x, v.y), m(v.z, v.w));
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-        return fmaxf(f.x, f.y);
-    }
-    __device__ static __forceinline__ void put(uint4 &o, int i, float lo, float hi) {
-        const __half2 r = __floats2half2_rn(lo, hi);
-        set_word(o, i, *reinterpret_cast<const unsigned int *>(&r));
+    __device__ static __forceinline__ uint4 put(const float (&x)[N]) {
+        uint4 o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) set_word(o, i, bits(__floats2half2_rn(x[2 * i], x[2 * i + 1])));
+        return o;
     }
     static constexpr unsigned int LOWEST = 0xfc00fc00u;
 };
 
-// ---- rows by clusters, a unit of 1024 logits by a warp ------------------------------------------------
+// ---- rows by clusters, a unit of 4096 bytes by a warp ---------------------------------------------------
 
-constexpr int UNIT = 1024;
+constexpr int UB = 4096;                    // a unit's bytes: eight chunks a lane
+constexpr int KU = UB / 512;
+template <class T> constexpr int UNIT = UB / (int)sizeof(T);   // and logits
 constexpr int MAX_WARPS = 16;      // with the one that answers
 constexpr int WAIT_TRIES = 1 << 22;   // of a bounded wait
 
 // How a launch lays its rows out: C blocks of W warps a row, R units of shared memory a warp, `rows_at_once` rows
 // in flight. Nothing in a row's results depends on it: a unit is always one warp's, in the same order of additions, and
 // the units are put together in theirs.
-struct Layout { int C, W, R, rows_at_once, units; bool resident; };
+struct Layout { int C, W, R, rows_at_once, table; bool resident; };   // table: places for a row's sums
 
 // The row's logits in memory: what lies before the first 16-byte boundary and behind the last (the edge, at most 14 logits), and
 // whole 16-byte chunks in between, in units.
@@ -247,9 +231,9 @@ template <class T> struct RowSpan {
         x = row + head;
         bytes = ((V - head) * (int)sizeof(T)) & ~15;
         tail = V - head - bytes / (int)sizeof(T);
-        units = (bytes + UNIT * (int)sizeof(T) - 1) / (UNIT * (int)sizeof(T));
+        units = (bytes + UB - 1) / UB;
     }
-    __device__ __forceinline__ int unit_bytes(int u) const { return min(bytes - u * UNIT * (int)sizeof(T), UNIT * (int)sizeof(T)); }
+    __device__ __forceinline__ int unit_bytes(int u) const { return min(bytes - u * UB, UB); }
     __device__ __forceinline__ bool edge() const { return head + tail > 0; }
     // the edge's logit of a lane: the first lanes have the head, those from 16 on the tail; -1 if it has none
     __device__ __forceinline__ int edge_at(int lane) const {
@@ -278,12 +262,11 @@ __device__ __forceinline__ double warp_sum(double v) {
 // 2^t for t <= 0 without ex2's bias: the nearest integer apart, the Taylor series of 2^f = e^(f ln 2) for the rest (|f| <= 1/2; the first term
 // left out is below 6e-9 of the sum).
 __device__ __forceinline__ float exp2_series(float t) {
-    if (!(t > -126.0f)) return t != t ? t : 0.0f;
-    const float n = rintf(t), f = __fmul_rn(t - n, 0.693147180559945f);
+    const float n = rintf(t < -127.0f ? -127.0f : t), f = __fmul_rn(t < -127.0f ? 0.0f : __fsub_rn(t, n), 0.693147180559945f);
     float p = 1.0f / 5040.0f;
     p = __fmaf_rn(p, f, 1.0f / 720.0f); p = __fmaf_rn(p, f, 1.0f / 120.0f); p = __fmaf_rn(p, f, 1.0f / 24.0f);
     p = __fmaf_rn(p, f, 1.0f / 6.0f); p = __fmaf_rn(p, f, 0.5f); p = __fmaf_rn(p, f, 1.0f); p = __fmaf_rn(p, f, 1.0f);
-    return p * __int_as_float(((int)n + 127) << 23);
+    return p * __int_as_float(((int)n + 127) << 23);   // 0 from 2^-127 down; NaN stays in p
 }
 
 // ex2.approx is low by 5.2e-8 in the mean, alike in every binade (4 million arguments from -32 to 0), which a sum of many terms
@@ -292,40 +275,40 @@ constexpr float EX2_LOW = 5.2e-8f;
 
 struct Stat { float m, s, w; unsigned int late; };   // maximum, sum, weighted sum of a unit; a wait that ran out
 
-template <class T, bool ENT>
-__device__ __forceinline__ Stat unit_stat(const uint4 (&v)[UNIT * sizeof(T) / 512], float c) {
-    constexpr int K = UNIT * sizeof(T) / 512, P = Chunk<T>::N / 2;
-    uint4 most = v[0];
+// A unit's, from shared memory twice: once for its maximum, then for the sums (four of either a lane).
+template <class T, bool ENT, bool FULL>
+__device__ __forceinline__ Stat unit_stat(const uint4 *slot, int chunks, float c) {
+    const int lane = threadIdx.x & 31;
+    constexpr unsigned int low = Chunk<T>::LOWEST;
+    uint4 most = make_uint4(low, low, low, low);
 #pragma unroll
-    for (int i = 1; i < K; i++) most = Chunk<T>::most2(most, v[i]);
+    for (int k = 0; k < KU; k++)
+        if (FULL || k * 32 + lane < chunks) {
+            const uint4 v = slot[k * 32 + lane];
+            most = make_uint4(Chunk<T>::max(most.x, v.x), Chunk<T>::max(most.y, v.y), Chunk<T>::max(most.z, v.z), Chunk<T>::max(most.w, v.w));
+        }
     Stat o;
-    o.m = warp_max(Chunk<T>::most(most));
+    o.m = warp_max(Chunk<T>::top(Chunk<T>::max(Chunk<T>::max(most.x, most.y), Chunk<T>::max(most.z, most.w))));
     o.late = 0;
     const float m = o.m == -INFINITY ? 0.0f : o.m;   // nothing but -inf (and NaN): sums of 0 (and NaN)
-    const f32x2 minus_m = pack2(-m, -m), cc = pack2(c, c);
-    f32x2 s = 0, w = 0;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < K; i++)
+    for (int k = 0; k < KU; k++)
+        if (FULL || k * 32 + lane < chunks) {
+            float x[Chunk<T>::N];
+            Chunk<T>::get(slot[k * 32 + lane], x);
 #pragma unroll
-        for (int j = 0; j < P; j++) {
-            const f32x2 d = add2(Chunk<T>::pair(v[i], j), minus_m);
-            float lo, hi;
-            unpack2(mul2(d, cc), lo, hi);
-            const f32x2 e = pack2(ex2(lo), ex2(hi));
-            s = add2(s, e);
-            if (ENT) {
-                unpack2(d, lo, hi);
-                w = fma2(e, pack2(lo < DEEP ? DEEP : lo, hi < DEEP ? DEEP : hi), w);
+            for (int i = 0; i < Chunk<T>::N; i++) {
+                const float d = __fsub_rn(x[i], m), e = ex2(d * c);
+                s[i & 3] += e;
+                if (ENT) w[i & 3] = __fmaf_rn(e, d < DEEP ? DEEP : d, w[i & 3]);
             }
         }
-    float lo, hi;
-    unpack2(s, lo, hi);
-    const float sum = warp_sum(lo + hi);
+    const float sum = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
     o.s = o.m == -INFINITY ? sum : __fmaf_rn(EX2_LOW, sum - 1.0f, sum);
     o.w = 0.0f;
     if (ENT) {
-        unpack2(w, lo, hi);
-        const float ws = warp_sum(lo + hi);
+        const float ws = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
         o.w = __fmaf_rn(EX2_LOW, ws, ws);
     }
     return o;
@@ -342,24 +325,36 @@ template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) 
     return o;
 }
 
-// All units of a row: a warp, the units in turn over the lanes, in 64 bits.
-template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, double &S, double &W, unsigned int &late) {
+// All units of a row: a warp, the units in turn over the lanes. (Sums in 64 bits: the tree adds numbers of one size.)
+template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, double &S, float &W, unsigned int &late) {
     const int lane = threadIdx.x & 31;
+    constexpr int HELD = 5;   // units a lane (160 a row: 327680 logits of 16 bits) that stay in registers
+    Stat v[HELD];
     float m = -INFINITY;
     unsigned int l = 0;
-    for (int u = lane; u < n; u += 32) { m = fmaxf(m, st[u].m); l |= st[u].late; }
+#pragma unroll
+    for (int k = 0; k < HELD; k++) {
+        v[k] = Stat{-INFINITY, 0.0f, 0.0f, 0};
+        if (k * 32 + lane < n) v[k] = st[k * 32 + lane];
+        m = fmaxf(m, v[k].m);
+        l |= v[k].late;
+    }
+    for (int u = HELD * 32 + lane; u < n; u += 32) { m = fmaxf(m, st[u].m); l |= st[u].late; }
     M = warp_max(m);
     late = __reduce_or_sync(0xffffffffu, l);
-    double s = 0.0, w = 0.0;
-    for (int u = lane; u < n; u += 32) {
-        const Stat o = st[u];
+    double s = 0.0;
+    float w = 0.0f;
+    const auto add = [&](const Stat &o) {
         const float d = o.m == -INFINITY ? 0.0f : __fsub_rn(o.m, M);   // (a unit of -inf: sums of 0, or NaN)
-        const double f = (double)exp2_series(d * c);
-        s += f * (double)o.s;
-        if (ENT) w += f * ((double)o.w + (double)(d < DEEP ? DEEP : d) * (double)o.s);
-    }
+        const float f = exp2_series(d * c);
+        s += (double)(f * o.s);
+        if (ENT) w = __fmaf_rn(f, __fmaf_rn(d < DEEP ? DEEP : d, o.s, o.w), w);
+    };
+#pragma unroll
+    for (int k = 0; k < HELD; k++) add(v[k]);
+    for (int u = HELD * 32 + lane; u < n; u += 32) add(st[u]);
     S = warp_sum(s);
-    W = ENT ? warp_sum(w) : 0.0;
+    W = ENT ? warp_sum(w) : 0.0f;
 }
 
 template <class T, bool ENT>
@@ -369,39 +364,26 @@ __device__ __forceinline__ float gradient_of(float x, float M, float c, float A,
 }
 
 // One unit's gradient: `to` is where its first logit's goes.
-template <class T, bool ENT>
-__device__ __forceinline__ void unit_gradient(const uint4 *slot, int bytes, T *to, bool wide, float M, float c, float A, float H) {
-    constexpr int K = UNIT * sizeof(T) / 512, N = Chunk<T>::N;
-    const int lane = threadIdx.x & 31, chunks = bytes >> 4;
-    const f32x2 minus_M = pack2(-M, -M), cc = pack2(c, c), aa = pack2(-A, -A), hh = pack2(-H, -H);
+template <class T, bool ENT, bool FULL>
+__device__ __forceinline__ void unit_gradient(const uint4 *slot, int chunks, T *to, bool wide, float M, float c, float A, float H) {
+    constexpr int N = Chunk<T>::N;
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < K; i++) {
-        const int k = i * 32 + lane;
-        if (k >= chunks) break;
-        const uint4 v = slot[k];
-        uint4 o;
+    for (int k = 0; k < KU; k++)
+        if (FULL || k * 32 + lane < chunks) {
+            float x[N];
+            Chunk<T>::get(slot[k * 32 + lane], x);
 #pragma unroll
-        for (int j = 0; j < N / 2; j++) {
-            const f32x2 d = add2(Chunk<T>::pair(v, j), minus_M);
-            float lo, hi;
-            unpack2(mul2(d, cc), lo, hi);
-            const f32x2 e = pack2(ex2(lo), ex2(hi));
-            f32x2 g = aa;
-            if (ENT) {
-                unpack2(d, lo, hi);
-                g = fma2(hh, pack2(lo < DEEP ? DEEP : lo, hi < DEEP ? DEEP : hi), aa);
+            for (int i = 0; i < N; i++) x[i] = gradient_of<T, ENT>(x[i], M, c, A, H);
+            const uint4 o = Chunk<T>::put(x);
+            if (wide) {
+                __stcs(reinterpret_cast<uint4 *>(to) + k * 32 + lane, o);
+            } else {
+                const T *e = reinterpret_cast<const T *>(&o);
+#pragma unroll
+                for (int i = 0; i < N; i++) to[(k * 32 + lane) * N + i] = e[i];
             }
-            unpack2(mul2(e, g), lo, hi);
-            Chunk<T>::put(o, j, lo, hi);
         }
-        if (wide) {
-            __stcs(reinterpret_cast<uint4 *>(to) + k, o);
-        } else {
-            const T *e = reinterpret_cast<const T *>(&o);
-#pragma unroll
-            for (int j = 0; j < N; j++) to[k * N + j] = e[j];
-        }
-    }
 }
 
 __device__ __forceinline__ uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
@@ -443,26 +425,50 @@ template <bool STATS> __device__ __forceinline__ bool row_read(const LossArgs &a
     return !(token < 0 || token >= a.V || (a.g_logprob[r] == 0.0f && !(a.g_entropy && a.g_entropy[r] != 0.0f)) || a.in_stats[2 * r + 1] == 0.0f);
 }
 
+// A bounded wait for a phase of a barrier to end (all lanes alike). A try lets the warp sleep for up to a microsecond: without the hint the
+// warps that waited took half of the issue slots.
+__device__ __forceinline__ bool wait_for(uint64_t *bar, int parity) {
+    bool here = false;
+    for (int i = 0; i < WAIT_TRIES && !here; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        here = ok != 0;
+    }
+    return __all_sync(0xffffffffu, here);
+}
+
 // A warp's units of shared memory, filled in the order in which it will want them, row after row.
 template <class T, bool STATS, bool GRAD> struct Feed {
     const LossArgs &a; const Layout &L;
-    uint4 *slots; uint64_t *bars;
-    int warp, warps;           // of the row's
+    const uint4 *slots; uint64_t *bars;
+    int warp, stride;          // of the row's warps; bytes from one of its units to the next
     int row0, step;            // this cluster's rows are row0, row0 + step, ...
     int i, base; unsigned int mask;   // the row that is being fetched, and which of 32 rows are read
-    int u, pass;               // its next unit, and which time through the row
+    const char *src; int left; // its next unit, and the bytes from there to the row's end
+    bool again_too;            // the row is fetched a second time
     int ahead;                 // units fetched or on their way, not given back
     int put, get, parity;      // slots
-    RowSpan<T> span;
     bool more, late;
     int owed, owed_slot, owed_parity;   // copies on their way when a wait ran out
 
-    __device__ __forceinline__ Feed(const LossArgs &a_, const Layout &L_, uint4 *s, uint64_t *b, int w, int ws, int r0, int st)
-        : a(a_), L(L_), slots(s), bars(b), warp(w), warps(ws), row0(r0), step(st), i(-1), base(-32), mask(0), u(0), pass(0), ahead(0), put(0), get(0), parity(0),
-          span((const T *)a_.logits, a_.V), more(true), late(false), owed(0) { next_row(); }
+    __device__ __forceinline__ Feed(const LossArgs &a_, const Layout &L_, const uint4 *s, uint64_t *b, int w, int ws, int r0, int st)
+        : a(a_), L(L_), slots(s), bars(b), warp(w), stride(ws * UB), row0(r0), step(st), i(-1), base(-32), mask(0), src(nullptr), left(0), again_too(false),
+          ahead(0), put(0), get(0), parity(0), more(true), late(false), owed(0) {
+        next_row();
+        while (more && ahead < L.R) fetch();
+    }
     __device__ __forceinline__ bool row_ok(int k) const { return (long long)row0 + (long long)k * step < a.B; }
+    __device__ __forceinline__ void start_row() {
+        const RowSpan<T> span((const T *)a.logits + (long long)(row0 + i * step) * a.row_stride, a.V);
+        src = (const char *)span.x + warp * UB;
+        left = span.bytes - warp * UB;
+    }
     __device__ void next_row() {
-        for (;;) {
+        do {
             i++;
             if (!row_ok(i)) { more = false; return; }
             if (i - base >= 32) {
@@ -470,60 +476,54 @@ template <class T, bool STATS, bool GRAD> struct Feed {
                 const int lane = threadIdx.x & 31;
                 mask = __ballot_sync(0xffffffffu, row_ok(i + lane) && row_read<STATS>(a, row0 + (i + lane) * step));
             }
-            if (!(mask >> (i - base) & 1)) continue;
-            span = RowSpan<T>((const T *)a.logits + (long long)(row0 + i * step) * a.row_stride, a.V);
-            u = warp; pass = 0;
-            if (u < span.units) return;
-        }
+            left = 0;
+            if (mask >> (i - base) & 1) start_row();
+        } while (left <= 0);
+        again_too = STATS && GRAD && !L.resident;
     }
-    // as many units as there is room for
+    // one more unit, where there is room
     __device__ __forceinline__ void fetch() {
-        while (more && ahead < L.R) {
-            if ((threadIdx.x & 31) == 0) {
-                const int bytes = span.unit_bytes(u);
-                mbar_expect_tx(&bars[put], (uint32_t)bytes);
-                bulk_g2s(slots + (size_t)put * (UNIT * sizeof(T) / 16), span.x + (size_t)u * UNIT, (uint32_t)bytes, &bars[put]);
-            }
-            ahead++;
-            if (++put == L.R) put = 0;
-            u += warps;
-            if (u >= span.units) {
-                if (STATS && GRAD && !L.resident && pass == 0) { pass = 1; u = warp; }
-                else next_row();
-            }
+        if (!more || ahead >= L.R) return;
+        if ((threadIdx.x & 31) == 0) {
+            const uint32_t bytes = (uint32_t)min(left, UB);
+            mbar_expect_tx(&bars[put], bytes);
+            bulk_g2s(const_cast<uint4 *>(slots) + put * (UB / 16), src, bytes, &bars[put]);
+        }
+        ahead++;
+        put = put + 1 == L.R ? 0 : put + 1;
+        src += stride;
+        left -= stride;
+        if (left <= 0) {
+            if (again_too) { again_too = false; start_row(); }
+            else next_row();
         }
     }
-    __device__ __forceinline__ const uint4 *slot(int k) const { return slots + (size_t)k * (UNIT * sizeof(T) / 16); }
-    // the k-th unit from the oldest that has not been given back has arrived
+    // the k-th unit from the oldest that has not been given back: when it has arrived, or as it was
     __device__ __forceinline__ const uint4 *wait(int k) {
         int s = get + k, p = parity;
         if (s >= L.R) { s -= L.R; p ^= 1; }
-        if (!late) {
-            bool here = false;
-            for (int i = 0; i < WAIT_TRIES && !here; i++) here = mbar_try_wait(&bars[s], p);
-            if (__any_sync(0xffffffffu, !here)) lose(k);
-        }
-        return slot(s);
+        if (!late && !wait_for(&bars[s], p)) lose(k);
+        return slots + s * (UB / 16);
+    }
+    __device__ __forceinline__ const uint4 *oldest() const { return slots + get * (UB / 16); }
+    __device__ __forceinline__ void give_back() {
+        __syncwarp();
+        ahead--;
+        if (++get == L.R) { get = 0; parity ^= 1; }
+        fetch();
     }
     // a wait ran out, with the units from the k-th on still on their way: nothing more is waited for or fetched
-    __device__ void lose(int k = 0) {
+    __device__ __forceinline__ void lose(int k = 0) {
         late = true; more = false;
         owed = ahead - k; owed_slot = get + k; owed_parity = parity;
         if (owed_slot >= L.R) { owed_slot -= L.R; owed_parity ^= 1; }
     }
     // before the block's shared memory goes back, what is on its way is waited for once more
-    __device__ void drain() {
+    __device__ __forceinline__ void drain() {
         for (; late && owed > 0; owed--) {
-            bool here = false;
-            for (int i = 0; i < WAIT_TRIES && !here; i++) here = mbar_try_wait(&bars[owed_slot], owed_parity);
+            wait_for(&bars[owed_slot], owed_parity);
             if (++owed_slot == L.R) { owed_slot = 0; owed_parity ^= 1; }
         }
-    }
-    __device__ __forceinline__ const uint4 *again(int k) const { int s = get + k; if (s >= L.R) s -= L.R; return slot(s); }
-    __device__ __forceinline__ void give_back() {
-        __syncwarp();
-        ahead--;
-        if (++get == L.R) { get = 0; parity ^= 1; }
     }
 };
 
@@ -532,7 +532,7 @@ template <class T, bool STATS, bool GRAD> struct Feed {
 // STATS: a row's maximum and sums, logprob, entropy and loss. GRAD: its gradient, from those (the policy loss) or, without
 // STATS, from the ones of an earlier pass. ENT: entropies take part.
 //
-// A warp has a ring of shared memory to itself and fills it with bulk copies, units of 1024 logits that only it reads: nothing
+// A warp has a ring of shared memory to itself and fills it with bulk copies, units of 4096 bytes that only it reads: nothing
 // waits for another warp but the row's sums. Where the row fits the rings of its cluster (resident) it is read from memory once: the units stay
 // until the gradient has been taken from them, and as they are given back the next row's come in, so reads and writes overlap.
 //
@@ -541,9 +541,9 @@ template <class T, bool STATS, bool GRAD> struct Feed {
 // ordinary warps' work, between two barriers, that took 12 of 29 thousand cycles a row.)
 constexpr int DEPTH = 4;   // rows whose sums may be on their way
 
-struct Control {
+struct alignas(16) Control {
     RowShare share[DEPTH];
-    uint64_t sums[DEPTH];      // all warps' sums of a row are there (used in the cluster's first block)
+    uint64_t sums[DEPTH];      // the sums of all of a row's units are there (used in the cluster's first block)
     uint64_t answered[DEPTH];  // ... and have been read, and `share` has what they came to
 };
 
@@ -556,35 +556,30 @@ __device__ __forceinline__ uint32_t at_rank(const void *p, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(p)), "r"(rank));
     return to;
 }
-__device__ __forceinline__ void put16(uint32_t to, float x, float y, float z, float w) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
-}
-__device__ __forceinline__ void arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// whether a phase of a barrier that other blocks arrive at has ended (all lanes alike)
-__device__ __forceinline__ bool wait_cluster(uint64_t *bar, int parity) {
-    bool here = false;
-    for (int i = 0; i < WAIT_TRIES && !here; i++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-        here = ok != 0;
+// 16 bytes into a block's shared memory. In a cluster of several they are counted by a barrier there, which needs no fence (one
+// would also wait for this thread's stores to global memory), and nobody may leave before all that is under way to it is there; a
+// block by itself stores them, and arrives at the barrier when it has.
+__device__ __forceinline__ void put16(bool alone, const void *at, int rank, float x, float y, float z, float w, const void *bar) {
+    if (alone) {
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(at)), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+    } else {
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at_rank(at, rank)),
+                     "r"(__float_as_uint(x)), "r"(__float_as_uint(y)), "r"(__float_as_uint(z)), "r"(__float_as_uint(w)), "r"(at_rank(bar, rank)) : "memory");
     }
-    return __all_sync(0xffffffffu, here);
+}
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-template <class T> size_t smem_of(const Layout &L) {
-    return (size_t)L.W * L.R * (UNIT * sizeof(T) + 8) + DEPTH * (size_t)(L.units + 1) * sizeof(Stat);
+size_t smem_of(const Layout &L) {
+    return (size_t)L.W * L.R * (UB + 8) + DEPTH * (size_t)L.table * sizeof(Stat);
 }
 
 // The warp that answers for the rows of a cluster.
 template <class T, bool GRAD, bool ENT>
 __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, Control &ctl, const Stat *stats, int row0, int step) {
     const int lane = threadIdx.x & 31;
+    const bool alone = L.C == 1;
     bool late = false;
     int n = 0;   // rows that are read
     RowIn mine = {};
@@ -602,7 +597,7 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
                     if (a.ref_logprob) mine.ref = a.ref_logprob[r];
                 }
                 if (mine.idle) row_idle(a, (int)r);
-                else if (mine.status) row_answer(a, (int)r, mine, 0.0f, 1.0, 0.0, 1.0f, true);
+                else if (mine.status) row_answer(a, (int)r, mine, 0.0f, 1.0, 0.0f, 1.0f, true);
             }
             mask = __ballot_sync(0xffffffffu, read);
         }
@@ -616,22 +611,22 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
         in.status = 0; in.idle = false;
         const RowSpan<T> span((const T *)a.logits + (long long)r * a.row_stride, a.V);
         const float c = LOG2E / in.T;
-        if (!late) late = !wait_cluster(&ctl.sums[s], (n / DEPTH) & 1);
-        float M;
-        double S, W;
+        const int units = span.units + (span.edge() ? 1 : 0);
+        if (lane == 0 && !alone) mbar_expect_tx(&ctl.sums[s], (uint32_t)(max(units, L.C * L.W) * (int)sizeof(Stat)));
+        if (!late) late = !wait_for(&ctl.sums[s], (n / DEPTH) & 1);
+        float M, W;
+        double S;
         unsigned int missed;
-        row_stat<ENT>(stats + s * (L.units + 1), span.units + (span.edge() ? 1 : 0), c, M, S, W, missed);
+        row_stat<ENT>(stats + s * L.table, units, c, M, S, W, missed);
         late = late || missed;   // (what was lost once has the barriers out of step)
         if (late) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
         const RowGrad q = row_answer(a, r, in, M, S, W, c, lane == 0);
         __syncwarp();
         if (lane < L.C) {
-            if (GRAD) {
-                const uint32_t to = at_rank(&ctl.share[s], lane);
-                put16(to, M, c, q.A, q.H);
-                put16(to + 16, q.token, __int_as_float(in.token), __int_as_float(q.A == 0.0f && q.H == 0.0f && q.token == 0.0f), 0.0f);
-            }
-            arrive(at_rank(&ctl.answered[s], lane));
+            put16(alone, &ctl.share[s], lane, M, c, q.A, q.H, &ctl.answered[s]);
+            put16(alone, &ctl.share[s].token_add, lane, q.token, __int_as_float(in.token),
+                  __int_as_float(q.A == 0.0f && q.H == 0.0f && q.token == 0.0f), 0.0f, &ctl.answered[s]);
+            if (alone) arrive(&ctl.answered[s]);
         }
         n++;
     }
@@ -641,16 +636,16 @@ template <class T, bool STATS, bool GRAD, bool ENT>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_constant__ LossArgs a, const __grid_constant__ Layout L) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ Control ctl;
-    constexpr int UB = UNIT * sizeof(T), K = UB / 512;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, rank = blockIdx.x % L.C;
     const int warp = rank * L.W + w, warps = L.C * L.W;
     const int row0 = blockIdx.x / L.C, step = L.rows_at_once;
+    const bool alone = L.C == 1;
     uint4 *slots = reinterpret_cast<uint4 *>(smem + (size_t)w * L.R * UB);
-    Stat *stats = reinterpret_cast<Stat *>(smem + (size_t)L.W * L.R * UB);   // [DEPTH][units + 1]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(stats + DEPTH * (L.units + 1)) + w * L.R;
+    Stat *stats = reinterpret_cast<Stat *>(smem + (size_t)L.W * L.R * UB);   // [DEPTH][table]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(stats + DEPTH * L.table) + w * L.R;
     if (STATS) {
         if (threadIdx.x < DEPTH) {
-            mbar_init(&ctl.sums[threadIdx.x], warps);
+            mbar_init(&ctl.sums[threadIdx.x], L.C == 1 ? warps : 1);
             mbar_init(&ctl.answered[threadIdx.x], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -666,7 +661,6 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         return;
     }
     Feed<T, STATS, GRAD> feed(a, L, slots, bars, warp, warps, row0, step);
-    feed.fetch();
     unsigned int mask = 0;
     RowShare mine = {};   // a row a lane: without STATS all of it, else c
     int n = 0;            // rows that are read
@@ -692,32 +686,31 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         if (STATS) {
             const int s = n % DEPTH;
             // without a gradient nobody waits for a row's answer: its table has to be free again
-            if (!GRAD && n >= DEPTH && !feed.late && !wait_cluster(&ctl.answered[s], (n / DEPTH + 1) & 1)) feed.lose();
-            const uint32_t st = at_rank(stats + s * (L.units + 1), 0);
+            if (!GRAD && n >= DEPTH && !feed.late && !wait_for(&ctl.answered[s], (n / DEPTH + 1) & 1)) feed.lose();
+            if (w == 0 && lane == 0 && !alone) mbar_expect_tx(&ctl.answered[s], (uint32_t)sizeof(RowShare));
+            const Stat *st = stats + s * L.table;
             int k = 0;
             for (int u = warp; u < span.units; u += warps) {
                 const uint4 *slot = feed.wait(k);
                 const int chunks = span.unit_bytes(u) >> 4;
-                uint4 v[K];
-#pragma unroll
-                for (int j = 0; j < K; j++) {
-                    constexpr unsigned int low = Chunk<T>::LOWEST;
-                    v[j] = j * 32 + lane < chunks ? slot[j * 32 + lane] : make_uint4(low, low, low, low);
-                }
-                Stat o = unit_stat<T, ENT>(v, q.c);
+                Stat o = chunks == UB / 16 ? unit_stat<T, ENT, true>(slot, chunks, q.c) : unit_stat<T, ENT, false>(slot, chunks, q.c);
                 o.late = feed.late || LOSS_KNOB(a, 16);   // (testing build: a wait that ran out)
-                if (lane == 0) put16(st + u * (uint32_t)sizeof(Stat), o.m, o.s, o.w, __uint_as_float(o.late));
+                if (lane == 0) put16(alone, st + u, 0, o.m, o.s, o.w, __uint_as_float(o.late), &ctl.sums[s]);
                 if (GRAD && L.resident) k++;
-                else { feed.give_back(); feed.fetch(); }
+                else feed.give_back();
             }
             if (edge_mine) {
                 const Stat o = edge_stat<ENT>(edge, q.c);
-                if (lane == 0) put16(st + span.units * (uint32_t)sizeof(Stat), o.m, o.s, o.w, 0.0f);
+                if (lane == 0) put16(alone, st + span.units, 0, o.m, o.s, o.w, 0.0f, &ctl.sums[s]);
             }
-            if (lane == 0) arrive(at_rank(&ctl.sums[s], 0));
+            // a warp without a unit says so: no row's answer may come before every warp is done with the row before it
+            if (lane == 0) {
+                if (alone) arrive(&ctl.sums[s]);
+                else if (warp >= span.units + (span.edge() ? 1 : 0)) put16(false, st + warp, 0, 0.0f, 0.0f, 0.0f, 0.0f, &ctl.sums[s]);
+            }
             n++;
             if (!GRAD) continue;
-            if (!feed.late && !wait_cluster(&ctl.answered[s], ((n - 1) / DEPTH) & 1)) feed.lose();
+            if (!feed.late && !wait_for(&ctl.answered[s], ((n - 1) / DEPTH) & 1)) feed.lose();
             q = ctl.share[s];
         } else {
             q.M = __shfl_sync(0xffffffffu, mine.M, from); q.A = __shfl_sync(0xffffffffu, mine.A, from); q.H = __shfl_sync(0xffffffffu, mine.H, from);
@@ -729,23 +722,26 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         const bool wide = ((uintptr_t)to & 15) == 0;
         if (q.zero) zero_row<T>(out, a.V, warp, warps);
         for (int u = warp; u < span.units; u += warps) {
-            const uint4 *slot = STATS && L.resident ? feed.again(0) : feed.wait(0);
+            const uint4 *slot = STATS && L.resident ? feed.oldest() : feed.wait(0);
             if (!q.zero) {
-                const int bytes = span.unit_bytes(u);
-                unit_gradient<T, ENT>(slot, bytes, to + (size_t)u * UNIT, wide, q.M, q.c, feed.late ? NAN : q.A, q.H);
-                const int t = q.token - span.head - u * UNIT;
-                if (t >= 0 && t < bytes / (int)sizeof(T)) {
+                const int chunks = span.unit_bytes(u) >> 4, t = q.token - span.head - u * UNIT<T>;
+                T *at = to + (size_t)u * UNIT<T>;
+                const float A = feed.late ? NAN : q.A;
+                if (wide && chunks == UB / 16) unit_gradient<T, ENT, true>(slot, chunks, at, true, q.M, q.c, A, q.H);
+                else unit_gradient<T, ENT, false>(slot, chunks, at, wide, q.M, q.c, A, q.H);
+                if (t >= 0 && t < chunks * Chunk<T>::N) {
                     __syncwarp();   // behind the store of the whole chunk
-                    if (lane == 0) to[(size_t)u * UNIT + t] = from_f32<T>(gradient_of<T, ENT>(to_f32(reinterpret_cast<const T *>(slot)[t]), q.M, q.c, q.A, q.H) + q.token_add);
+                    if (lane == 0) at[t] = from_f32<T>(gradient_of<T, ENT>(to_f32(reinterpret_cast<const T *>(slot)[t]), q.M, q.c, A, q.H) + q.token_add);
                 }
             }
             feed.give_back();
-            feed.fetch();
         }
         if (edge_at != INT32_MIN && !q.zero)
             to[edge_at] = from_f32<T>(gradient_of<T, ENT>(edge, q.M, q.c, q.A, q.H) + (edge_at == q.token - span.head ? q.token_add : 0.0f));
     }
     feed.drain();
+    if (STATS && w == 0)   // the last answers, which without a gradient nobody has waited for
+        for (int k = max(n - DEPTH, 0); k < n; k++) wait_for(&ctl.answered[k % DEPTH], (k / DEPTH) & 1);
     if (STATS) cluster_sync();   // nobody leaves while another block has something for it
 }
 
@@ -841,6 +837,8 @@ __global__ void __launch_bounds__(ST) pairs_kernel(const __grid_constant__ PairA
 constexpr int MAX_DEVICES = 64;
 constexpr size_t BLOCK_SMEM_2 = 112 * 1024, BLOCK_SMEM_1 = 224 * 1024;   // dynamic shared memory of two blocks an SM, and of one
 
+struct Fits { int threads, smem, n; };
+
 int sm_count_of(int &dev) {
     int sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { dev = -1; return 0; }
@@ -849,10 +847,9 @@ int sm_count_of(int &dev) {
 
 template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms, int &blocks_per_sm) {
     Layout L{};
-    const int UB = UNIT * (int)sizeof(T);
-    L.units = (V + UNIT - 1) / UNIT + 1;   // (an unaligned row's whole chunks, and its edge)
+    L.table = max((V + UNIT<T> - 1) / UNIT<T> + 1, 8 * MAX_WARPS);   // (an unaligned row's whole chunks, and its edge; a place a warp)
     const int most = (V * (int)sizeof(T) + UB - 1) / UB;
-    const int room2 = (int)((BLOCK_SMEM_2 - DEPTH * (size_t)(L.units + 1) * sizeof(Stat)) / (UB + 8)), room1 = (int)((BLOCK_SMEM_1 - DEPTH * (size_t)(L.units + 1) * sizeof(Stat)) / (UB + 8));
+    const int room2 = (int)((BLOCK_SMEM_2 - DEPTH * (size_t)L.table * sizeof(Stat)) / (UB + 8)), room1 = (int)((BLOCK_SMEM_1 - DEPTH * (size_t)L.table * sizeof(Stat)) / (UB + 8));
     int room = room2;
     blocks_per_sm = 2;
     L.C = 1;
@@ -881,24 +878,36 @@ template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(cons
     if (sms <= 0) return cudaErrorInvalidDevice;
     int per_sm = 1;
     Layout L = layout_of<T, STATS, GRAD>(a.B, a.V, sms, per_sm);
-    const size_t smem = smem_of<T>(L);
+    const size_t smem = smem_of(L);
     auto kernel = rows_kernel<T, STATS, GRAD, ENT>;
-    static bool asked[MAX_DEVICES] = {};
-    if (dev >= MAX_DEVICES || !asked[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BLOCK_SMEM_1);
-        if (e != cudaSuccess) return e;
-        if (dev < MAX_DEVICES) asked[dev] = true;
-    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
-    long long clusters = (long long)sms * per_sm / L.C;
-    if (clusters > a.B) clusters = a.B;
-    if (clusters < 1) clusters = 1;
-    L.rows_at_once = (int)clusters;
-    cfg.gridDim = dim3((unsigned int)(clusters * L.C)); cfg.blockDim = dim3(32u * (unsigned int)(L.W + (STATS ? 1 : 0))); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.blockDim = dim3(32u * (unsigned int)(L.W + (STATS ? 1 : 0))); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned int)L.C; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = STATS && L.C > 1 ? 1 : 0;
+    // How many clusters the device holds at a time, asked once per device and layout: one too many would wait for all
+    // rows of another (72 of four blocks, two an SM, fit where 74 would fill the SMs).
+    static thread_local Fits known[MAX_DEVICES][4] = {};
+    const int kind = L.C == 1 ? 0 : L.C == 2 ? 1 : L.C == 4 ? 2 : 3;
+    Fits fits = dev < MAX_DEVICES ? known[dev][kind] : Fits{};
+    if (fits.threads != (int)cfg.blockDim.x || fits.smem != (int)smem) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BLOCK_SMEM_1);
+        if (e != cudaSuccess) return e;
+        fits = Fits{(int)cfg.blockDim.x, (int)smem, 0};
+        if (cfg.numAttrs) {
+            cfg.gridDim = dim3((unsigned int)L.C);
+            e = cudaOccupancyMaxActiveClusters(&fits.n, kernel, &cfg);
+        } else {
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fits.n, kernel, (int)cfg.blockDim.x, smem);
+            fits.n = fits.n * sms / L.C;
+        }
+        if (e != cudaSuccess) return e;
+        if (fits.n < 1) return cudaErrorLaunchOutOfResources;
+        if (dev < MAX_DEVICES) known[dev][kind] = fits;
+    }
+    L.rows_at_once = fits.n < a.B ? fits.n : a.B;
+    cfg.gridDim = dim3((unsigned int)(L.rows_at_once * L.C));
     return cudaLaunchKernelEx(&cfg, kernel, a, (const Layout)L);
 }
 
