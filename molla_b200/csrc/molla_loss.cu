@@ -51,7 +51,7 @@ template <> __device__ __forceinline__ __half from_f32(float v) { return __float
 // A row's inputs; a lane fetches a row's, 32 rows ahead.
 struct RowIn {
     int token;
-    float T, old, advantage, weight, ref, xt;   // temperature; the policy loss's; the token's logit
+    float T, per_T, old, advantage, weight, ref, xt;   // temperature and its inverse; the policy loss's; the token's logit
     unsigned int status; // why the row cannot be answered, before it is read
     bool idle;           // nothing to answer: no token, or no weight
 };
@@ -60,6 +60,7 @@ __device__ __forceinline__ RowIn row_in(const LossArgs &a, int r) {
     RowIn in;
     in.token = a.tokens[r];
     in.T = a.temperature ? a.temperature[r] : 1.0f;
+    in.per_T = 1.0f / in.T;
     in.weight = a.weight ? a.weight[r] : 1.0f;
     in.old = in.advantage = in.ref = in.xt = 0.0f;
     in.idle = in.token == -1 || in.weight == 0.0f;
@@ -72,26 +73,36 @@ __device__ __forceinline__ RowIn row_in(const LossArgs &a, int r) {
     return in;
 }
 
-// The gradient's three numbers: add at the token, and A and H of the formula.
+// The gradient's three numbers: add at the token, and A and H of the formula; `mean` is W/(S T).
 struct RowGrad { float token, A, H; };
 
-__device__ __forceinline__ RowGrad row_grad(float g, float h, float T, float S, float w_over_st) {
+__device__ __forceinline__ RowGrad row_grad(float g, float h, float per_T, float per_S, float mean) {
     RowGrad o;
-    const float inv = 1.0f / (T * S);
-    o.token = g / T;
-    o.A = (g - h * w_over_st) * inv;
-    o.H = h * inv / T;
+    const float inv = per_T * per_S;
+    o.token = g * per_T;
+    o.A = __fmaf_rn(-h, mean, g) * inv;
+    o.H = h * inv * per_T;
     return o;
 }
 
-// ln S, S > 0: the power of two apart, the rest (within a factor of the square root of two of one) is below 0.35 and good to 3e-8
-// in 32 bits. (With log, exp and the divisions in 64 bits a row's scalars took 6200 cycles, in which its blocks wait.)
-__device__ __forceinline__ double ln_of(double S) {
-    if (!(S > 0.0) || isinf(S)) return S == 0.0 ? -INFINITY : S;   // (NaN stays)
-    int k = __double2hiint(S) - 0x3fe6a09e;   // the exponent of S / sqrt(1/2)
-    k >>= 20;
-    const double f = __hiloint2double(__double2hiint(S) - (k << 20), __double2loint(S));
-    return (double)k * 0.693147180559945309 + (double)log1pf((float)(f - 1.0));
+// A value in two floats, the second below the first's last bit.
+struct Two { float hi, lo; };
+__device__ __forceinline__ Two two_sum(float a, float b) {
+    const float s = __fadd_rn(a, b), bb = __fsub_rn(s, a);
+    return Two{s, __fadd_rn(__fsub_rn(a, __fsub_rn(s, bb)), __fsub_rn(b, bb))};
+}
+__device__ __forceinline__ bool ordinary(float x) { return fabsf(x) < 3e38f; }
+
+constexpr float LN2 = 0.693147180559945309f, LN2_LEFT = (float)(0.693147180559945309 - (double)LN2);
+constexpr float LN2_SHORT = 0.693145751953125f, LN2_REST = (float)(0.693147180559945309 - 0.693145751953125);   // 17 bits, times a small integer exact
+
+// ln S, S > 0: the power of two apart; what is left lies within a factor of the square root of two of one, its logarithm is below 0.35 and
+// good to 3e-8.
+__device__ __forceinline__ Two ln_of(float S) {
+    if (!(S > 0.0f) || !ordinary(S)) return Two{S == 0.0f ? -INFINITY : S, 0.0f};   // (NaN stays)
+    const int k = (__float_as_int(S) - 0x3f3504f3) >> 23;
+    const float y = log1pf(__fsub_rn(__int_as_float(__float_as_int(S) - (k << 23)), 1.0f)), n = (float)k;
+    return two_sum(n * LN2_SHORT, __fmaf_rn(n, LN2_REST, y));
 }
 
 // exp(q) - 1 - q: for small q from its series, which the difference would lose
@@ -104,41 +115,64 @@ __device__ __forceinline__ float exp_less_line(float q) {
     return p * q * q;
 }
 
-// What a row answers once its maximum M, sum S and, where entropies are wanted, W are known.
-__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, int r, const RowIn &in, float M, double S, float W, float c, bool write) {
-    const unsigned int status = in.status | (M == -INFINITY && S == 0.0 && !in.status ? MOLLA_ROW_EMPTY : 0u);
+// What a row answers once its maximum M, sum S and, where entropies are wanted, W are known: first what its gradient
+// waits for, all of it in 32 bits (conversions to 64 run where the exponentials do, behind theirs: with 64 bits, logarithm, exponential and
+// divisions a row's blocks waited 6200 cycles, with conversions alone 2400), then the rest.
+struct Answer { unsigned int status; Two l, lnS; float mean, ratio, q, kl; bool held; };
+
+template <bool ENT>
+__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in, float M, float S, float W, float c, Answer &o) {
+    o.status = in.status | (M == -INFINITY && S == 0.0f && !in.status ? MOLLA_ROW_EMPTY : 0u);
+    o.lnS = ln_of(S);
+    const float per_S = __frcp_rn(S);
     // ln p in the temperature that c stands for (log2(e)/T rounded): the error of c then moves ln S and the token together
-    const double to_nats = (double)c * 0.693147180559945309, lnS = ln_of(S);
-    const double l = ((double)in.xt - (double)M) * to_nats - lnS;
-    const float mean = W / (float)S * (float)to_nats;   // of (x - M)/T
-    const double H = lnS - (double)mean;
-    if (write) {
-        a.status[r] = status;
-        a.logprob[r] = status ? NAN : (float)l;
-        if (a.entropy) a.entropy[r] = status ? NAN : (float)H;
-        if (a.stats) { a.stats[2 * r] = status ? NAN : M; a.stats[2 * r + 1] = status ? 0.0f : (float)S; }
+    const float nats = c * LN2, nats_lo = __fadd_rn(__fmaf_rn(c, LN2, -nats), c * LN2_LEFT), dx = __fsub_rn(in.xt, M);
+    o.mean = ENT ? W * per_S * nats : 0.0f;
+    if (ordinary(dx) && ordinary(o.lnS.hi)) {
+        const Two d = two_sum(in.xt, -M);
+        const float p = dx * nats, p_lo = __fmaf_rn(dx, nats, -p) + __fmaf_rn(dx, nats_lo, d.lo * nats);
+        const Two s = two_sum(p, -o.lnS.hi);
+        o.l = two_sum(s.hi, s.lo + (p_lo - o.lnS.lo));
+    } else {
+        o.l = Two{dx * nats - o.lnS.hi, 0.0f};
     }
+    o.ratio = o.q = o.kl = 0.0f;
+    o.held = false;
     if (!a.row_loss) return RowGrad{0.0f, 0.0f, 0.0f};
-    // the policy loss
-    const double w = in.weight, adv = in.advantage;
-    const double ratio = expf((float)(l - (double)in.old));
-    const double lo = 1.0 - (double)a.clip_low, hi = 1.0 + (double)a.clip_high;
-    const double u = ratio * adv, v = fmin(fmax(ratio, lo), hi) * adv;
-    const bool held = v < u;
-    double term = -(held ? v : u), g = held ? 0.0 : -u;   // (a ratio that is NaN is not held)
+    o.ratio = expf((o.l.hi - in.old) + o.l.lo);
+    o.held = (in.advantage > 0.0f && o.ratio > 1.0f + a.clip_high) || (in.advantage < 0.0f && o.ratio < 1.0f - a.clip_low);   // (not a NaN)
+    float g = o.held ? 0.0f : -(o.ratio * in.advantage);
     if (a.ref_logprob) {
-        const float q = (float)((double)in.ref - l), kl = exp_less_line(q);
-        if (a.kl && write) a.kl[r] = status ? NAN : kl;
-        if (a.kl_coef != 0.0f) { term += (double)a.kl_coef * (double)kl; g -= (double)a.kl_coef * ((double)kl + (double)q); }
+        o.q = (in.ref - o.l.hi) - o.l.lo;
+        o.kl = exp_less_line(o.q);
+        if (a.kl_coef != 0.0f) g = __fmaf_rn(-a.kl_coef, o.kl + o.q, g);
     }
-    double h = 0.0;
-    if (a.entropy_coef != 0.0f) { term -= (double)a.entropy_coef * H; h = -w * (double)a.entropy_coef; }
-    if (write) {
-        a.row_loss[r] = status ? NAN : (float)(w * term);
-        if (a.clipped) a.clipped[r] = !status && held;
-    }
-    const double gs = (double)a.scale * (double)a.grad_scale;
-    return status ? RowGrad{0.0f, 0.0f, 0.0f} : row_grad((float)(g * w * gs), (float)(h * gs), in.T, (float)S, mean);
+    const float by = in.weight * a.scale * a.grad_scale;
+    return o.status ? RowGrad{0.0f, 0.0f, 0.0f} : row_grad(g * by, ENT ? -a.entropy_coef * by : 0.0f, in.per_T, per_S, o.mean);
+}
+
+__device__ __forceinline__ void row_write(const LossArgs &a, int r, const RowIn &in, float M, float S, const Answer &o) {
+    const unsigned int status = o.status;
+    const double H = ((double)o.lnS.hi + (double)o.lnS.lo) - (double)o.mean;
+    a.status[r] = status;
+    a.logprob[r] = status ? NAN : o.l.hi;
+    if (a.entropy) a.entropy[r] = status ? NAN : (float)H;
+    if (a.stats) { a.stats[2 * r] = status ? NAN : M; a.stats[2 * r + 1] = status ? 0.0f : S; }
+    if (!a.row_loss) return;
+    const double bound = o.held ? (in.advantage > 0.0f ? 1.0 + (double)a.clip_high : 1.0 - (double)a.clip_low) : (double)o.ratio;
+    double term = -bound * (double)in.advantage;
+    if (a.kl) a.kl[r] = status ? NAN : o.kl;
+    if (a.kl_coef != 0.0f) term += (double)a.kl_coef * (double)o.kl;
+    if (a.entropy_coef != 0.0f) term -= (double)a.entropy_coef * H;
+    a.row_loss[r] = status ? NAN : (float)((double)in.weight * term);
+    if (a.clipped) a.clipped[r] = !status && o.held;
+}
+
+// a row that cannot be answered, and is not read
+__device__ __forceinline__ void row_refused(const LossArgs &a, int r, const RowIn &in) {
+    Answer o = {};
+    o.status = in.status;
+    row_write(a, r, in, 0.0f, 1.0f, o);
 }
 
 __device__ void row_idle(const LossArgs &a, int r) {
@@ -218,7 +252,7 @@ constexpr int WAIT_TRIES = 1 << 22;   // of a bounded wait
 // How a launch lays its rows out: C blocks of W warps a row, R units of shared memory a warp, `rows_at_once` rows
 // in flight. Nothing in a row's results depends on it: a unit is always one warp's, in the same order of additions, and
 // the units are put together in theirs.
-struct Layout { int C, W, R, rows_at_once, table; bool resident; };   // table: places for a row's sums
+struct Layout { int C, W, R, rows_at_once, table; bool resident, ahead; };   // table: places for a row's sums
 
 // The row's logits in memory: what lies before the first 16-byte boundary and behind the last (the edge, at most 14 logits), and
 // whole 16-byte chunks in between, in units.
@@ -253,12 +287,6 @@ __device__ __forceinline__ float warp_sum(float v) {
     for (int i = 16; i > 0; i >>= 1) v += __shfl_xor_sync(0xffffffffu, v, i);
     return v;
 }
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) v += __shfl_xor_sync(0xffffffffu, v, i);
-    return v;
-}
-
 // 2^t for t <= 0 without ex2's bias: the nearest integer apart, the Taylor series of 2^f = e^(f ln 2) for the rest (|f| <= 1/2; the first term
 // left out is below 6e-9 of the sum).
 __device__ __forceinline__ float exp2_series(float t) {
@@ -325,10 +353,10 @@ template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) 
     return o;
 }
 
-// All units of a row: a warp, the units in turn over the lanes. (Sums in 64 bits: the tree adds numbers of one size.)
-template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, double &S, float &W, unsigned int &late) {
+// All units of a row: a warp, the units in turn over the lanes, then a tree.
+template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, float &S, float &W, unsigned int &late) {
     const int lane = threadIdx.x & 31;
-    constexpr int HELD = 5;   // units a lane (160 a row: 327680 logits of 16 bits) that stay in registers
+    constexpr int HELD = 3;   // units a lane that stay in registers
     Stat v[HELD];
     float m = -INFINITY;
     unsigned int l = 0;
@@ -341,20 +369,19 @@ template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int
     }
     for (int u = HELD * 32 + lane; u < n; u += 32) { m = fmaxf(m, st[u].m); l |= st[u].late; }
     M = warp_max(m);
-    late = __reduce_or_sync(0xffffffffu, l);
-    double s = 0.0;
-    float w = 0.0f;
+    late = __any_sync(0xffffffffu, l != 0);
+    S = W = 0.0f;
     const auto add = [&](const Stat &o) {
         const float d = o.m == -INFINITY ? 0.0f : __fsub_rn(o.m, M);   // (a unit of -inf: sums of 0, or NaN)
         const float f = exp2_series(d * c);
-        s += (double)(f * o.s);
-        if (ENT) w = __fmaf_rn(f, __fmaf_rn(d < DEEP ? DEEP : d, o.s, o.w), w);
+        S = __fmaf_rn(f, o.s, S);
+        if (ENT) W = __fmaf_rn(f, __fmaf_rn(d < DEEP ? DEEP : d, o.s, o.w), W);
     };
 #pragma unroll
     for (int k = 0; k < HELD; k++) add(v[k]);
     for (int u = HELD * 32 + lane; u < n; u += 32) add(st[u]);
-    S = warp_sum(s);
-    W = ENT ? warp_sum(w) : 0.0f;
+    S = warp_sum(S);
+    if (ENT) W = warp_sum(W);
 }
 
 template <class T, bool ENT>
@@ -410,7 +437,8 @@ __device__ __forceinline__ RowShare row_given(const LossArgs &a, int r) {
     o.token = a.tokens[r];
     o.M = a.in_stats[2 * r];
     o.c = LOG2E / T;
-    const RowGrad q = row_grad(g, h, T, S, h != 0.0f ? (float)(ln_of(S) - (double)a.in_entropy[r]) : 0.0f);
+    const Two lnS = ln_of(S);
+    const RowGrad q = row_grad(g, h, 1.0f / T, __frcp_rn(S), h != 0.0f ? (lnS.hi - a.in_entropy[r]) + lnS.lo : 0.0f);
     o.A = q.A; o.H = q.H; o.token_add = q.token;
     return o;
 }
@@ -448,38 +476,56 @@ template <class T, bool STATS, bool GRAD> struct Feed {
     int warp, stride;          // of the row's warps; bytes from one of its units to the next
     int row0, step;            // this cluster's rows are row0, row0 + step, ...
     int i, base; unsigned int mask;   // the row that is being fetched, and which of 32 rows are read
-    const char *src; int left; // its next unit, and the bytes from there to the row's end
-    bool again_too;            // the row is fetched a second time
+    int row, before;           // the row and the one before it, -1 where there is none
+    const char *src; int left; // the next unit, and the bytes from there to its row's end
+    bool second;               // it is one of the row before, for the gradient
     int ahead;                 // units fetched or on their way, not given back
     int put, get, parity;      // slots
     bool more, late;
     int owed, owed_slot, owed_parity;   // copies on their way when a wait ran out
 
     __device__ __forceinline__ Feed(const LossArgs &a_, const Layout &L_, const uint4 *s, uint64_t *b, int w, int ws, int r0, int st)
-        : a(a_), L(L_), slots(s), bars(b), warp(w), stride(ws * UB), row0(r0), step(st), i(-1), base(-32), mask(0), src(nullptr), left(0), again_too(false),
+        : a(a_), L(L_), slots(s), bars(b), warp(w), stride(ws * UB), row0(r0), step(st), i(-1), base(-32), mask(0), row(-1), before(-1), src(nullptr), left(0), second(true),
           ahead(0), put(0), get(0), parity(0), more(true), late(false), owed(0) {
-        next_row();
+        next();
         while (more && ahead < L.R) fetch();
     }
     __device__ __forceinline__ bool row_ok(int k) const { return (long long)row0 + (long long)k * step < a.B; }
-    __device__ __forceinline__ void start_row() {
-        const RowSpan<T> span((const T *)a.logits + (long long)(row0 + i * step) * a.row_stride, a.V);
+    __device__ __forceinline__ void start(int r) {
+        const RowSpan<T> span((const T *)a.logits + (long long)r * a.row_stride, a.V);
         src = (const char *)span.x + warp * UB;
         left = span.bytes - warp * UB;
     }
-    __device__ void next_row() {
-        do {
+    // The next row that is read, or -1.
+    __device__ int next_row() {
+        for (;;) {
             i++;
-            if (!row_ok(i)) { more = false; return; }
+            if (!row_ok(i)) return -1;
             if (i - base >= 32) {
                 base = i;
                 const int lane = threadIdx.x & 31;
                 mask = __ballot_sync(0xffffffffu, row_ok(i + lane) && row_read<STATS>(a, row0 + (i + lane) * step));
             }
+            if (mask >> (i - base) & 1) return row0 + i * step;
+        }
+    }
+    // From the end of one row's units to the first of another: a row for its sums, then, where units do not stay (see rows_kernel), the row before
+    // it for its gradient.
+    __device__ void next() {
+        do {
+            if (STATS && GRAD && !L.resident && !second) {
+                second = true;
+                const int r = L.ahead ? before : row;
+                if (r >= 0) { start(r); continue; }
+            }
+            before = row;
+            row = before < 0 && i >= 0 ? -1 : next_row();
+            second = row < 0;
             left = 0;
-            if (mask >> (i - base) & 1) start_row();
+            if (row >= 0) start(row);
+            else if (STATS && GRAD && !L.resident && L.ahead && before >= 0) start(before);
+            else { more = false; return; }
         } while (left <= 0);
-        again_too = STATS && GRAD && !L.resident;
     }
     // one more unit, where there is room
     __device__ __forceinline__ void fetch() {
@@ -493,10 +539,7 @@ template <class T, bool STATS, bool GRAD> struct Feed {
         put = put + 1 == L.R ? 0 : put + 1;
         src += stride;
         left -= stride;
-        if (left <= 0) {
-            if (again_too) { again_too = false; start_row(); }
-            else next_row();
-        }
+        if (left <= 0) next();
     }
     // the k-th unit from the oldest that has not been given back: when it has arrived, or as it was
     __device__ __forceinline__ const uint4 *wait(int k) {
@@ -534,11 +577,11 @@ template <class T, bool STATS, bool GRAD> struct Feed {
 //
 // A warp has a ring of shared memory to itself and fills it with bulk copies, units of 4096 bytes that only it reads: nothing
 // waits for another warp but the row's sums. Where the row fits the rings of its cluster (resident) it is read from memory once: the units stay
-// until the gradient has been taken from them, and as they are given back the next row's come in, so reads and writes overlap.
+// until the gradient has been taken from them; else they come a second time, out of L2. The sums of a row come before the gradient of the
+// row before it, whose answer arrives meanwhile, so that nobody waits for an answer.
 //
-// The sums of all units go to the cluster's first block, where one warp does nothing but put them together, answer for the row and
-// tell the gradient's numbers to all blocks; it has fetched the rows' inputs beforehand. (As a part of one of the
-// ordinary warps' work, between two barriers, that took 12 of 29 thousand cycles a row.)
+// The sums of all units go to every block that waits for the row's answer; one warp there does nothing but put them together and answer; it has fetched
+// the rows' inputs beforehand. (As a part of one of the ordinary warps' work, between two barriers, that took 12 of 29 thousand cycles a row.)
 constexpr int DEPTH = 4;   // rows whose sums may be on their way
 
 struct alignas(16) Control {
@@ -575,11 +618,11 @@ size_t smem_of(const Layout &L) {
     return (size_t)L.W * L.R * (UB + 8) + DEPTH * (size_t)L.table * sizeof(Stat);
 }
 
-// The warp that answers for the rows of a cluster.
+// The warp that answers for the rows of a cluster: one in every block where a gradient waits, else one in the first.
 template <class T, bool GRAD, bool ENT>
-__device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, Control &ctl, const Stat *stats, int row0, int step) {
+__device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, Control &ctl, Stat *stats, int rank, int row0, int step) {
     const int lane = threadIdx.x & 31;
-    const bool alone = L.C == 1;
+    const bool alone = L.C == 1, first = rank == 0;
     bool late = false;
     int n = 0;   // rows that are read
     RowIn mine = {};
@@ -591,20 +634,22 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
             if (r < a.B) {
                 mine = row_in(a, (int)r);
                 read = !mine.idle && !mine.status;
-                if (read) mine.xt = to_f32(((const T *)a.logits)[r * a.row_stride + mine.token]);
+                if (read && first) mine.xt = to_f32(((const T *)a.logits)[r * a.row_stride + mine.token]);
                 if (a.row_loss) {
                     mine.old = a.old_logprob[r]; mine.advantage = a.advantage[r];
                     if (a.ref_logprob) mine.ref = a.ref_logprob[r];
                 }
-                if (mine.idle) row_idle(a, (int)r);
-                else if (mine.status) row_answer(a, (int)r, mine, 0.0f, 1.0, 0.0f, 1.0f, true);
+                if (first && mine.idle) row_idle(a, (int)r);
+                else if (first && mine.status) row_refused(a, (int)r, mine);
             }
             mask = __ballot_sync(0xffffffffu, read);
         }
         if (!(mask >> (i % 32) & 1)) continue;
         const int r = row0 + i * step, from = i % 32, s = n % DEPTH;
+        Stat *st = stats + s * L.table;
         RowIn in;
         in.token = __shfl_sync(0xffffffffu, mine.token, from); in.T = __shfl_sync(0xffffffffu, mine.T, from);
+        in.per_T = __shfl_sync(0xffffffffu, mine.per_T, from);
         in.old = __shfl_sync(0xffffffffu, mine.old, from); in.advantage = __shfl_sync(0xffffffffu, mine.advantage, from);
         in.weight = __shfl_sync(0xffffffffu, mine.weight, from); in.ref = __shfl_sync(0xffffffffu, mine.ref, from);
         in.xt = __shfl_sync(0xffffffffu, mine.xt, from);
@@ -612,24 +657,35 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
         const RowSpan<T> span((const T *)a.logits + (long long)r * a.row_stride, a.V);
         const float c = LOG2E / in.T;
         const int units = span.units + (span.edge() ? 1 : 0);
-        if (lane == 0 && !alone) mbar_expect_tx(&ctl.sums[s], (uint32_t)(max(units, L.C * L.W) * (int)sizeof(Stat)));
+        // The token's logit is the first block's to fetch: where the gradient takes the logits' place nobody may write before it has been read,
+        // and nobody does before it has the answer, which needs it.
+        if (!alone) {
+            if (lane == 0) mbar_expect_tx(&ctl.sums[s], (uint32_t)((max(units, L.C * L.W) + (GRAD ? 1 : 0)) * (int)sizeof(Stat)));
+            if (GRAD && first && lane < L.C) put16(false, st + L.table - 1, lane, in.xt, 0.0f, 0.0f, 0.0f, &ctl.sums[s]);
+        }
         if (!late) late = !wait_for(&ctl.sums[s], (n / DEPTH) & 1);
-        float M, W;
-        double S;
+        if (GRAD && !alone) in.xt = st[L.table - 1].m;
+        float M, S, W;
         unsigned int missed;
-        row_stat<ENT>(stats + s * L.table, units, c, M, S, W, missed);
+        row_stat<ENT>(st, units, c, M, S, W, missed);
         late = late || missed;   // (what was lost once has the barriers out of step)
         if (late) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
-        const RowGrad q = row_answer(a, r, in, M, S, W, c, lane == 0);
+        Answer o;
+        const RowGrad q = row_answer<ENT>(a, in, M, S, W, c, o);
         __syncwarp();
-        if (lane < L.C) {
-            put16(alone, &ctl.share[s], lane, M, c, q.A, q.H, &ctl.answered[s]);
-            put16(alone, &ctl.share[s].token_add, lane, q.token, __int_as_float(in.token),
-                  __int_as_float(q.A == 0.0f && q.H == 0.0f && q.token == 0.0f), 0.0f, &ctl.answered[s]);
-            if (alone) arrive(&ctl.answered[s]);
+        if (GRAD || alone) {
+            if (lane == 0) {
+                ctl.share[s] = RowShare{M, c, q.A, q.H, q.token, in.token, q.A == 0.0f && q.H == 0.0f && q.token == 0.0f, 0};
+                arrive(&ctl.answered[s]);
+            }
+        } else if (lane < L.C) {   // nothing but the news that the table is free again
+            put16(false, &ctl.share[s], lane, 0.0f, 0.0f, 0.0f, 0.0f, &ctl.answered[s]);
         }
+        if (first && lane == 0) row_write(a, r, in, M, S, o);
         n++;
     }
+    if (late)   // what is still on its way to this block
+        for (int k = max(n - DEPTH, 0); k < n; k++) wait_for(&ctl.sums[k % DEPTH], (k / DEPTH) & 1);
 }
 
 template <class T, bool STATS, bool GRAD, bool ENT>
@@ -656,7 +712,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
     if (STATS) cluster_sync();
     else __syncwarp();
     if (STATS && w == L.W) {
-        if (rank == 0) answer_rows<T, GRAD, ENT>(a, L, ctl, stats, row0, step);
+        if (GRAD || rank == 0) answer_rows<T, GRAD, ENT>(a, L, ctl, stats, rank, row0, step);
         cluster_sync();
         return;
     }
@@ -664,62 +720,73 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
     unsigned int mask = 0;
     RowShare mine = {};   // a row a lane: without STATS all of it, else c
     int n = 0;            // rows that are read
-    for (int i = 0; feed.row_ok(i); i++) {
+    int held = 0;         // units that stay for the gradient of the row before
+    int before = -1;      // that row
+    for (int i = 0;; i++) {
         const int r = row0 + i * step, from = i % 32;
-        if (from == 0) {
+        const bool last = !feed.row_ok(i);
+        if (last && before < 0) break;
+        if (from == 0 && !last) {
             const bool ok = feed.row_ok(i + lane), read = ok && row_read<STATS>(a, row0 + (i + lane) * step);
             mask = __ballot_sync(0xffffffffu, read);
             if (!STATS && read) mine = row_given(a, row0 + (i + lane) * step);
             if (STATS) mine.c = LOG2E / (read && a.temperature ? a.temperature[row0 + (i + lane) * step] : 1.0f);
         }
-        T *out = GRAD ? (T *)a.grad + (long long)r * a.grad_stride : nullptr;
-        if (!(mask >> from & 1)) {
-            if (GRAD) zero_row<T>(out, a.V, warp, warps);
+        if (!last && !(mask >> from & 1)) {
+            if (GRAD) zero_row<T>((T *)a.grad + (long long)r * a.grad_stride, a.V, warp, warps);
             continue;
         }
-        const RowSpan<T> span((const T *)a.logits + (long long)r * a.row_stride, a.V);
-        const bool edge_mine = span.edge() && warp == span.units % warps;
-        const int edge_at = edge_mine ? span.edge_at(lane) : INT32_MIN;
-        const float edge = edge_at != INT32_MIN ? to_f32(span.x[edge_at]) : -INFINITY;
-        RowShare q;
-        q.c = __shfl_sync(0xffffffffu, mine.c, from);
-        if (STATS) {
+        int units = 0;   // of this row that stay
+        if (STATS && !last) {
+            const RowSpan<T> span((const T *)a.logits + (long long)r * a.row_stride, a.V);
             const int s = n % DEPTH;
+            const float c = __shfl_sync(0xffffffffu, mine.c, from);
             // without a gradient nobody waits for a row's answer: its table has to be free again
             if (!GRAD && n >= DEPTH && !feed.late && !wait_for(&ctl.answered[s], (n / DEPTH + 1) & 1)) feed.lose();
-            if (w == 0 && lane == 0 && !alone) mbar_expect_tx(&ctl.answered[s], (uint32_t)sizeof(RowShare));
+            if (!GRAD && w == 0 && lane == 0 && !alone) mbar_expect_tx(&ctl.answered[s], 16);
             const Stat *st = stats + s * L.table;
-            int k = 0;
+            const bool tell = lane < (GRAD ? L.C : 1);   // a lane a block that wants to know
             for (int u = warp; u < span.units; u += warps) {
-                const uint4 *slot = feed.wait(k);
+                const uint4 *slot = feed.wait(held + units);
                 const int chunks = span.unit_bytes(u) >> 4;
-                Stat o = chunks == UB / 16 ? unit_stat<T, ENT, true>(slot, chunks, q.c) : unit_stat<T, ENT, false>(slot, chunks, q.c);
+                Stat o = chunks == UB / 16 ? unit_stat<T, ENT, true>(slot, chunks, c) : unit_stat<T, ENT, false>(slot, chunks, c);
                 o.late = feed.late || LOSS_KNOB(a, 16);   // (testing build: a wait that ran out)
-                if (lane == 0) put16(alone, st + u, 0, o.m, o.s, o.w, __uint_as_float(o.late), &ctl.sums[s]);
-                if (GRAD && L.resident) k++;
+                if (tell) put16(alone, st + u, lane, o.m, o.s, o.w, __uint_as_float(o.late), &ctl.sums[s]);
+                if (GRAD && L.resident) units++;
                 else feed.give_back();
             }
-            if (edge_mine) {
-                const Stat o = edge_stat<ENT>(edge, q.c);
-                if (lane == 0) put16(alone, st + span.units, 0, o.m, o.s, o.w, 0.0f, &ctl.sums[s]);
+            if (span.edge() && warp == span.units % warps) {
+                const int at = span.edge_at(lane);
+                const Stat o = edge_stat<ENT>(at != INT32_MIN ? to_f32(span.x[at]) : -INFINITY, c);
+                if (tell) put16(alone, st + span.units, lane, o.m, o.s, o.w, 0.0f, &ctl.sums[s]);
             }
-            // a warp without a unit says so: no row's answer may come before every warp is done with the row before it
-            if (lane == 0) {
-                if (alone) arrive(&ctl.sums[s]);
-                else if (warp >= span.units + (span.edge() ? 1 : 0)) put16(false, st + warp, 0, 0.0f, 0.0f, 0.0f, 0.0f, &ctl.sums[s]);
-            }
+            // a warp without a unit says so: no row's answer may come before every warp is done with the rows before it
+            __syncwarp();
+            if (alone) { if (lane == 0) arrive(&ctl.sums[s]); }
+            else if (tell && warp >= span.units + (span.edge() ? 1 : 0)) put16(false, st + warp, lane, 0.0f, 0.0f, 0.0f, 0.0f, &ctl.sums[s]);
             n++;
-            if (!GRAD) continue;
-            if (!feed.late && !wait_for(&ctl.answered[s], ((n - 1) / DEPTH) & 1)) feed.lose();
+        }
+        if (!GRAD) continue;
+        // The gradient: of the row before, whose answer came meanwhile (of this one where it is given)
+        int g = r;
+        if (STATS && L.ahead) { g = before; before = last ? -1 : r; held = units; }
+        if (g < 0) continue;
+        RowShare q;
+        if (STATS) {
+            const int k = last || !L.ahead ? n - 1 : n - 2, s = k % DEPTH;
+            if (!feed.late && !wait_for(&ctl.answered[s], (k / DEPTH) & 1)) feed.lose();
             q = ctl.share[s];
         } else {
-            q.M = __shfl_sync(0xffffffffu, mine.M, from); q.A = __shfl_sync(0xffffffffu, mine.A, from); q.H = __shfl_sync(0xffffffffu, mine.H, from);
+            q.M = __shfl_sync(0xffffffffu, mine.M, from); q.c = __shfl_sync(0xffffffffu, mine.c, from);
+            q.A = __shfl_sync(0xffffffffu, mine.A, from); q.H = __shfl_sync(0xffffffffu, mine.H, from);
             q.token_add = __shfl_sync(0xffffffffu, mine.token_add, from); q.token = __shfl_sync(0xffffffffu, mine.token, from);
             q.zero = 0;
         }
-        if (!GRAD) continue;
-        T *to = out + span.head;
+        const RowSpan<T> span((const T *)a.logits + (long long)g * a.row_stride, a.V);
+        T *out = (T *)a.grad + (long long)g * a.grad_stride, *to = out + span.head;
         const bool wide = ((uintptr_t)to & 15) == 0;
+        const int edge_at = span.edge() && warp == span.units % warps ? span.edge_at(lane) : INT32_MIN;
+        const float edge = edge_at != INT32_MIN ? to_f32(span.x[edge_at]) : 0.0f;
         if (q.zero) zero_row<T>(out, a.V, warp, warps);
         for (int u = warp; u < span.units; u += warps) {
             const uint4 *slot = STATS && L.resident ? feed.oldest() : feed.wait(0);
@@ -847,7 +914,7 @@ int sm_count_of(int &dev) {
 
 template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms, int &blocks_per_sm) {
     Layout L{};
-    L.table = max((V + UNIT<T> - 1) / UNIT<T> + 1, 8 * MAX_WARPS);   // (an unaligned row's whole chunks, and its edge; a place a warp)
+    L.table = max((V + UNIT<T> - 1) / UNIT<T> + 1, 8 * MAX_WARPS) + 1;   // (an unaligned row's whole chunks, and its edge; a place a warp; the token's logit)
     const int most = (V * (int)sizeof(T) + UB - 1) / UB;
     const int room2 = (int)((BLOCK_SMEM_2 - DEPTH * (size_t)L.table * sizeof(Stat)) / (UB + 8)), room1 = (int)((BLOCK_SMEM_1 - DEPTH * (size_t)L.table * sizeof(Stat)) / (UB + 8));
     int room = room2;
@@ -868,6 +935,7 @@ template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms
     const int each = (most + L.C * L.W - 1) / (L.C * L.W);
     L.R = room / L.W;
     if (L.R > 64) L.R = 64;
+    L.ahead = 2 * each <= L.R;
     L.resident = each <= L.R;
     return L;
 }
