@@ -257,7 +257,7 @@ struct Layout { int C, W, R, rows_at_once, table; bool resident, ahead; };   // 
 // The row's logits in memory: what lies before the first 16-byte boundary and behind the last (the edge, at most 14 logits), and
 // whole 16-byte chunks in between, in units.
 template <class T> struct RowSpan {
-    const T *x; int head, units, tail; int bytes;
+    const T *x; int head, units, full, tail; int bytes;
     __device__ __forceinline__ RowSpan(const T *row, int V) {
         const int off = (int)((uintptr_t)row & 15);
         head = off ? (16 - off) / (int)sizeof(T) : 0;
@@ -266,8 +266,9 @@ template <class T> struct RowSpan {
         bytes = ((V - head) * (int)sizeof(T)) & ~15;
         tail = V - head - bytes / (int)sizeof(T);
         units = (bytes + UB - 1) / UB;
+        full = bytes / UB;
     }
-    __device__ __forceinline__ int unit_bytes(int u) const { return min(bytes - u * UB, UB); }
+    __device__ __forceinline__ int last_chunks() const { return (bytes - full * UB) >> 4; }   // of the unit that is not full
     __device__ __forceinline__ bool edge() const { return head + tail > 0; }
     // the edge's logit of a lane: the first lanes have the head, those from 16 on the tail; -1 if it has none
     __device__ __forceinline__ int edge_at(int lane) const {
@@ -301,18 +302,38 @@ __device__ __forceinline__ float exp2_series(float t) {
 // keeps: uncorrected, the log ratio of a sequence of 200 rows was off by 1e-5. Its value at 0 is exact.
 constexpr float EX2_LOW = 5.2e-8f;
 
+// 16 bytes of shared memory by their address there (pointers into it cost 64-bit arithmetic)
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+template <class T> __device__ __forceinline__ float lds_element(uint32_t at);
+template <> __device__ __forceinline__ float lds_element<float>(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned short lds2(uint32_t at) {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    return v;
+}
+template <> __device__ __forceinline__ float lds_element<__nv_bfloat16>(uint32_t at) { return __uint_as_float((unsigned int)lds2(at) << 16); }
+template <> __device__ __forceinline__ float lds_element<__half>(uint32_t at) { return __half2float(__ushort_as_half(lds2(at))); }
+
 struct Stat { float m, s, w; unsigned int late; };   // maximum, sum, weighted sum of a unit; a wait that ran out
 
 // A unit's, from shared memory twice: once for its maximum, then for the sums (four of either a lane).
 template <class T, bool ENT, bool FULL>
-__device__ __forceinline__ Stat unit_stat(const uint4 *slot, int chunks, float c) {
+__device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
     const int lane = threadIdx.x & 31;
     constexpr unsigned int low = Chunk<T>::LOWEST;
     uint4 most = make_uint4(low, low, low, low);
-#pragma unroll
+#pragma unroll(FULL ? KU / 2 : 1)
     for (int k = 0; k < KU; k++)
         if (FULL || k * 32 + lane < chunks) {
-            const uint4 v = slot[k * 32 + lane];
+            const uint4 v = lds16(slot + k * 512 + lane * 16);
             most = make_uint4(Chunk<T>::max(most.x, v.x), Chunk<T>::max(most.y, v.y), Chunk<T>::max(most.z, v.z), Chunk<T>::max(most.w, v.w));
         }
     Stat o;
@@ -320,11 +341,11 @@ __device__ __forceinline__ Stat unit_stat(const uint4 *slot, int chunks, float c
     o.late = 0;
     const float m = o.m == -INFINITY ? 0.0f : o.m;   // nothing but -inf (and NaN): sums of 0 (and NaN)
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
+#pragma unroll(FULL ? KU / 2 : 1)
     for (int k = 0; k < KU; k++)
         if (FULL || k * 32 + lane < chunks) {
             float x[Chunk<T>::N];
-            Chunk<T>::get(slot[k * 32 + lane], x);
+            Chunk<T>::get(lds16(slot + k * 512 + lane * 16), x);
 #pragma unroll
             for (int i = 0; i < Chunk<T>::N; i++) {
                 const float d = __fsub_rn(x[i], m), e = ex2(d * c);
@@ -392,14 +413,14 @@ __device__ __forceinline__ float gradient_of(float x, float M, float c, float A,
 
 // One unit's gradient: `to` is where its first logit's goes.
 template <class T, bool ENT, bool FULL>
-__device__ __forceinline__ void unit_gradient(const uint4 *slot, int chunks, T *to, bool wide, float M, float c, float A, float H) {
+__device__ __forceinline__ void unit_gradient(uint32_t slot, int chunks, T *to, bool wide, float M, float c, float A, float H) {
     constexpr int N = Chunk<T>::N;
     const int lane = threadIdx.x & 31;
-#pragma unroll
+#pragma unroll(FULL ? KU / 2 : 1)
     for (int k = 0; k < KU; k++)
         if (FULL || k * 32 + lane < chunks) {
             float x[N];
-            Chunk<T>::get(slot[k * 32 + lane], x);
+            Chunk<T>::get(lds16(slot + k * 512 + lane * 16), x);
 #pragma unroll
             for (int i = 0; i < N; i++) x[i] = gradient_of<T, ENT>(x[i], M, c, A, H);
             const uint4 o = Chunk<T>::put(x);
@@ -453,26 +474,46 @@ template <bool STATS> __device__ __forceinline__ bool row_read(const LossArgs &a
     return !(token < 0 || token >= a.V || (a.g_logprob[r] == 0.0f && !(a.g_entropy && a.g_entropy[r] != 0.0f)) || a.in_stats[2 * r + 1] == 0.0f);
 }
 
-// A bounded wait for a phase of a barrier to end (all lanes alike). A try lets the warp sleep for up to a microsecond: without the hint the
-// warps that waited took half of the issue slots.
-__device__ __forceinline__ bool wait_for(uint64_t *bar, int parity) {
-    bool here = false;
-    for (int i = 0; i < WAIT_TRIES && !here; i++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-        here = ok != 0;
+// A bulk copy of global memory to shared, with what L2 is told about the lines: nothing, that they will be read once more before long, or
+// that this is the last time.
+enum Lines { ANY, KEEP, LAST };
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar, Lines lines) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+    if (lines == ANY) {
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                     : "memory");
+    } else {
+        uint64_t policy;
+        if (lines == KEEP) asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
+        else asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(dst), "l"(src),
+                     "r"(bytes), "r"(bar), "l"(policy)
+                     : "memory");
     }
-    return __all_sync(0xffffffffu, here);
 }
+
+// A bounded wait for a phase of a barrier to end (all lanes alike). A try lets the warp sleep for up to a microsecond.
+__device__ __forceinline__ bool try_for(uint32_t bar, int parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
+}
+__device__ __forceinline__ bool wait_for(uint32_t bar, int parity) {
+    if (try_for(bar, parity)) return true;
+    for (int i = 0; i < WAIT_TRIES; i++)
+        if (try_for(bar, parity)) return true;
+    return false;
+}
+__device__ __forceinline__ bool wait_for(uint64_t *bar, int parity) { return wait_for(smem_u32(bar), parity); }
 
 // A warp's units of shared memory, filled in the order in which it will want them, row after row.
 template <class T, bool STATS, bool GRAD> struct Feed {
     const LossArgs &a; const Layout &L;
-    const uint4 *slots; uint64_t *bars;
+    uint32_t slots, bars;      // in shared memory
     int warp, stride;          // of the row's warps; bytes from one of its units to the next
     int row0, step;            // this cluster's rows are row0, row0 + step, ...
     int i, base; unsigned int mask;   // the row that is being fetched, and which of 32 rows are read
@@ -484,7 +525,7 @@ template <class T, bool STATS, bool GRAD> struct Feed {
     bool more, late;
     int owed, owed_slot, owed_parity;   // copies on their way when a wait ran out
 
-    __device__ __forceinline__ Feed(const LossArgs &a_, const Layout &L_, const uint4 *s, uint64_t *b, int w, int ws, int r0, int st)
+    __device__ __forceinline__ Feed(const LossArgs &a_, const Layout &L_, uint32_t s, uint32_t b, int w, int ws, int r0, int st)
         : a(a_), L(L_), slots(s), bars(b), warp(w), stride(ws * UB), row0(r0), step(st), i(-1), base(-32), mask(0), row(-1), before(-1), src(nullptr), left(0), second(true),
           ahead(0), put(0), get(0), parity(0), more(true), late(false), owed(0) {
         next();
@@ -531,9 +572,10 @@ template <class T, bool STATS, bool GRAD> struct Feed {
     __device__ __forceinline__ void fetch() {
         if (!more || ahead >= L.R) return;
         if ((threadIdx.x & 31) == 0) {
-            const uint32_t bytes = (uint32_t)min(left, UB);
-            mbar_expect_tx(&bars[put], bytes);
-            bulk_g2s(const_cast<uint4 *>(slots) + put * (UB / 16), src, bytes, &bars[put]);
+            const uint32_t to = slots + put * UB, bar = bars + put * 8, bytes = (uint32_t)min(left, UB);
+            if (!(STATS && GRAD) || L.resident) bulk_copy(to, src, bytes, bar, ANY);
+            else if (second) bulk_copy(to, src, bytes, bar, LAST);
+            else bulk_copy(to, src, bytes, bar, KEEP);
         }
         ahead++;
         put = put + 1 == L.R ? 0 : put + 1;
@@ -542,13 +584,13 @@ template <class T, bool STATS, bool GRAD> struct Feed {
         if (left <= 0) next();
     }
     // the k-th unit from the oldest that has not been given back: when it has arrived, or as it was
-    __device__ __forceinline__ const uint4 *wait(int k) {
+    __device__ __forceinline__ uint32_t wait(int k) {
         int s = get + k, p = parity;
         if (s >= L.R) { s -= L.R; p ^= 1; }
-        if (!late && !wait_for(&bars[s], p)) lose(k);
-        return slots + s * (UB / 16);
+        if (!late && !wait_for(bars + s * 8, p)) lose(k);
+        return slots + s * UB;
     }
-    __device__ __forceinline__ const uint4 *oldest() const { return slots + get * (UB / 16); }
+    __device__ __forceinline__ uint32_t oldest() const { return slots + get * UB; }
     __device__ __forceinline__ void give_back() {
         __syncwarp();
         ahead--;
@@ -564,7 +606,7 @@ template <class T, bool STATS, bool GRAD> struct Feed {
     // before the block's shared memory goes back, what is on its way is waited for once more
     __device__ __forceinline__ void drain() {
         for (; late && owed > 0; owed--) {
-            wait_for(&bars[owed_slot], owed_parity);
+            wait_for(bars + owed_slot * 8, owed_parity);
             if (++owed_slot == L.R) { owed_slot = 0; owed_parity ^= 1; }
         }
     }
@@ -696,7 +738,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
     const int warp = rank * L.W + w, warps = L.C * L.W;
     const int row0 = blockIdx.x / L.C, step = L.rows_at_once;
     const bool alone = L.C == 1;
-    uint4 *slots = reinterpret_cast<uint4 *>(smem + (size_t)w * L.R * UB);
+    const uint32_t slots = smem_u32(smem) + w * L.R * UB;
     Stat *stats = reinterpret_cast<Stat *>(smem + (size_t)L.W * L.R * UB);   // [DEPTH][table]
     uint64_t *bars = reinterpret_cast<uint64_t *>(stats + DEPTH * L.table) + w * L.R;
     if (STATS) {
@@ -716,7 +758,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         cluster_sync();
         return;
     }
-    Feed<T, STATS, GRAD> feed(a, L, slots, bars, warp, warps, row0, step);
+    Feed<T, STATS, GRAD> feed(a, L, slots, smem_u32(bars), warp, warps, row0, step);
     unsigned int mask = 0;
     RowShare mine = {};   // a row a lane: without STATS all of it, else c
     int n = 0;            // rows that are read
@@ -747,9 +789,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
             const Stat *st = stats + s * L.table;
             const bool tell = lane < (GRAD ? L.C : 1);   // a lane a block that wants to know
             for (int u = warp; u < span.units; u += warps) {
-                const uint4 *slot = feed.wait(held + units);
-                const int chunks = span.unit_bytes(u) >> 4;
-                Stat o = chunks == UB / 16 ? unit_stat<T, ENT, true>(slot, chunks, c) : unit_stat<T, ENT, false>(slot, chunks, c);
+                const uint32_t slot = feed.wait(held + units);
+                Stat o = u < span.full ? unit_stat<T, ENT, true>(slot, 0, c) : unit_stat<T, ENT, false>(slot, span.last_chunks(), c);
                 o.late = feed.late || LOSS_KNOB(a, 16);   // (testing build: a wait that ran out)
                 if (tell) put16(alone, st + u, lane, o.m, o.s, o.w, __uint_as_float(o.late), &ctl.sums[s]);
                 if (GRAD && L.resident) units++;
@@ -788,17 +829,19 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         const int edge_at = span.edge() && warp == span.units % warps ? span.edge_at(lane) : INT32_MIN;
         const float edge = edge_at != INT32_MIN ? to_f32(span.x[edge_at]) : 0.0f;
         if (q.zero) zero_row<T>(out, a.V, warp, warps);
-        for (int u = warp; u < span.units; u += warps) {
-            const uint4 *slot = STATS && L.resident ? feed.oldest() : feed.wait(0);
+        const int at_token = q.token - span.head, token_unit = at_token < 0 ? -1 : at_token / UNIT<T>;
+        T *at = to + warp * UNIT<T>;
+        for (int u = warp; u < span.units; u += warps, at += warps * UNIT<T>) {
+            const uint32_t slot = STATS && L.resident ? feed.oldest() : feed.wait(0);
+            const float A = feed.late ? NAN : q.A;
             if (!q.zero) {
-                const int chunks = span.unit_bytes(u) >> 4, t = q.token - span.head - u * UNIT<T>;
-                T *at = to + (size_t)u * UNIT<T>;
-                const float A = feed.late ? NAN : q.A;
-                if (wide && chunks == UB / 16) unit_gradient<T, ENT, true>(slot, chunks, at, true, q.M, q.c, A, q.H);
-                else unit_gradient<T, ENT, false>(slot, chunks, at, wide, q.M, q.c, A, q.H);
-                if (t >= 0 && t < chunks * Chunk<T>::N) {
+                if (u < span.full && wide) unit_gradient<T, ENT, true>(slot, 0, at, true, q.M, q.c, A, q.H);
+                else unit_gradient<T, ENT, false>(slot, u < span.full ? UB / 16 : span.last_chunks(), at, wide, q.M, q.c, A, q.H);
+                if (u == token_unit) {
+                    const int t = at_token - u * UNIT<T>;
                     __syncwarp();   // behind the store of the whole chunk
-                    if (lane == 0) at[t] = from_f32<T>(gradient_of<T, ENT>(to_f32(reinterpret_cast<const T *>(slot)[t]), q.M, q.c, A, q.H) + q.token_add);
+                    if (lane == 0 && t * (int)sizeof(T) < span.bytes - u * UB)
+                        at[t] = from_f32<T>(gradient_of<T, ENT>(lds_element<T>(slot + t * (int)sizeof(T)), q.M, q.c, A, q.H) + q.token_add);
                 }
             }
             feed.give_back();
@@ -902,7 +945,6 @@ __global__ void __launch_bounds__(ST) pairs_kernel(const __grid_constant__ PairA
 // ---- launches --------------------------------------------------------------------------------------------
 
 constexpr int MAX_DEVICES = 64;
-constexpr size_t BLOCK_SMEM_2 = 112 * 1024, BLOCK_SMEM_1 = 224 * 1024;   // dynamic shared memory of two blocks an SM, and of one
 
 struct Fits { int threads, smem, n; };
 
@@ -912,40 +954,40 @@ int sm_count_of(int &dev) {
     return sms;
 }
 
-template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms, int &blocks_per_sm) {
+constexpr size_t block_smem(int blocks_per_sm) { return (size_t)(blocks_per_sm == 1 ? 224 : blocks_per_sm == 2 ? 112 : blocks_per_sm == 3 ? 74 : 55) * 1024; }
+
+// C blocks a row, W warps a block or as many fewer as share its units evenly (6 % of the rounds idle), and the shared memory of
+// `per_sm` blocks an SM.
+Layout layout_with(int C, int W, int per_sm, int V, int size) {
     Layout L{};
-    L.table = max((V + UNIT<T> - 1) / UNIT<T> + 1, 8 * MAX_WARPS) + 1;   // (an unaligned row's whole chunks, and its edge; a place a warp; the token's logit)
-    const int most = (V * (int)sizeof(T) + UB - 1) / UB;
-    const int room2 = (int)((BLOCK_SMEM_2 - DEPTH * (size_t)L.table * sizeof(Stat)) / (UB + 8)), room1 = (int)((BLOCK_SMEM_1 - DEPTH * (size_t)L.table * sizeof(Stat)) / (UB + 8));
-    int room = room2;
-    blocks_per_sm = 2;
-    L.C = 1;
-    if (STATS && GRAD) {
-        while (L.C < 8 && 4 * most > 3 * room2 * L.C) L.C *= 2;
-        if (most > room2 * L.C) { room = room1; blocks_per_sm = 1; }
-    }
-    while (L.C < 8 && (long long)B * L.C * 2 * 9 <= (long long)sms * blocks_per_sm * 8 && most > L.C * 8) L.C *= 2;
-    // as many warps as share the row's units most evenly
+    const int unit = UB / size, most = (int)(((long long)V * size + UB - 1) / UB), share = (most + C - 1) / C;   // units of a row, and of a block
+    L.C = C;
+    L.table = max((V + unit - 1) / unit + 1, C * W) + 1;   // (an unaligned row's whole chunks and its edge, or a place a warp; the token's logit)
+    const int slots = (int)((block_smem(per_sm) - DEPTH * (size_t)L.table * sizeof(Stat)) / (UB + 8));
+    if (W > share) W = share > 0 ? share : 1;
+    if (W > slots) W = slots;
     int best = 0x7fffffff;
-    for (int w = STATS ? MAX_WARPS - 1 : MAX_WARPS; w >= 6; w--) {
-        const int slots = (most + L.C * w - 1) / (L.C * w) * L.C * w;
-        if (slots < best) { best = slots; L.W = w; }
+    for (int w = W; w > W / 2; w--) {
+        const int rounds = (share + w - 1) / w * w;
+        if (rounds < best && (best == 0x7fffffff || best * 16 > share * 17)) { best = rounds; L.W = w; }
     }
-    if (L.W > most) L.W = most > 0 ? most : 1;
-    const int each = (most + L.C * L.W - 1) / (L.C * L.W);
-    L.R = room / L.W;
-    if (L.R > 64) L.R = 64;
+    const int each = (share + L.W - 1) / L.W;
+    L.R = slots / L.W;
+    if (L.R > 32) L.R = 32;
     L.ahead = 2 * each <= L.R;
     L.resident = each <= L.R;
     return L;
+}
+
+template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms) {
+    return layout_with(1, STATS ? 13 : 16, 2, V, (int)sizeof(T));
 }
 
 template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(const LossArgs &a, cudaStream_t st) {
     int dev = 0;
     const int sms = sm_count_of(dev);
     if (sms <= 0) return cudaErrorInvalidDevice;
-    int per_sm = 1;
-    Layout L = layout_of<T, STATS, GRAD>(a.B, a.V, sms, per_sm);
+    Layout L = layout_of<T, STATS, GRAD>(a.B, a.V, sms);
     const size_t smem = smem_of(L);
     auto kernel = rows_kernel<T, STATS, GRAD, ENT>;
     cudaLaunchConfig_t cfg = {};
@@ -960,7 +1002,7 @@ template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(cons
     const int kind = L.C == 1 ? 0 : L.C == 2 ? 1 : L.C == 4 ? 2 : 3;
     Fits fits = dev < MAX_DEVICES ? known[dev][kind] : Fits{};
     if (fits.threads != (int)cfg.blockDim.x || fits.smem != (int)smem) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BLOCK_SMEM_1);
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)block_smem(1));
         if (e != cudaSuccess) return e;
         fits = Fits{(int)cfg.blockDim.x, (int)smem, 0};
         if (cfg.numAttrs) {
