@@ -31,6 +31,9 @@ constexpr float LOG2E = (float)LOG2E_64;
 constexpr float DEEP = -1e30f;    // where x - M is held, so that 0 * (x - M) is 0 for logits of -inf too
 constexpr unsigned int ROW_ERRORS = MOLLA_ROW_BAD_TOKEN | MOLLA_ROW_EMPTY | MOLLA_ROW_INVALID_CONFIG | MOLLA_ROW_LOAD_TIMEOUT;
 
+// Kernels of one call begin when the one before is about to end, and wait here until it has.
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -738,6 +741,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
     const int warp = rank * L.W + w, warps = L.C * L.W;
     const int row0 = blockIdx.x / L.C, step = L.rows_at_once;
     const bool alone = L.C == 1;
+    wait_for_launch_before();
     const uint32_t slots = smem_u32(smem) + w * L.R * UB;
     Stat *stats = reinterpret_cast<Stat *>(smem + (size_t)L.W * L.R * UB);   // [DEPTH][table]
     uint64_t *bars = reinterpret_cast<uint64_t *>(stats + DEPTH * L.table) + w * L.R;
@@ -873,6 +877,7 @@ __device__ double sum_1024(double v, double *ws) {
 
 __global__ void __launch_bounds__(ST) row_sum_kernel(const float *row_loss, int B, float scale, float *loss) {
     __shared__ double ws[ST / 32];
+    wait_for_launch_before();
     double v = 0.0;
     for (int i = threadIdx.x; i < B; i += ST) v += (double)row_loss[i];
     v = sum_1024(v, ws);
@@ -899,6 +904,7 @@ __device__ __forceinline__ double sigmoid(double m) { return m >= 0.0 ? 1.0 / (1
 // One block: the pairs a warp each, in turn.
 __global__ void __launch_bounds__(ST) pairs_kernel(const __grid_constant__ PairArgs a) {
     __shared__ double ws[ST / 32];
+    wait_for_launch_before();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, S = 2 * a.n_pairs;
     int bad = 0;
     for (int s = threadIdx.x; s < S; s += ST) bad |= a.off[s] < 0 || a.off[s + 1] < a.off[s] || a.off[s + 1] > a.B;
@@ -954,7 +960,7 @@ int sm_count_of(int &dev) {
     return sms;
 }
 
-constexpr size_t block_smem(int blocks_per_sm) { return (size_t)(blocks_per_sm == 1 ? 224 : blocks_per_sm == 2 ? 112 : blocks_per_sm == 3 ? 74 : 55) * 1024; }
+constexpr size_t block_smem(int per_sm) { return (size_t)(228 / per_sm - 2) * 1024; }   // of a block's dynamic shared memory: an SM's 228 KB less what each block takes besides
 
 // C blocks a row, W warps a block or as many fewer as share its units evenly (6 % of the rounds idle), and the shared memory of
 // `per_sm` blocks an SM.
@@ -964,7 +970,7 @@ Layout layout_with(int C, int W, int per_sm, int V, int size) {
     L.C = C;
     L.table = max((V + unit - 1) / unit + 1, C * W) + 1;   // (an unaligned row's whole chunks and its edge, or a place a warp; the token's logit)
     const int slots = (int)((block_smem(per_sm) - DEPTH * (size_t)L.table * sizeof(Stat)) / (UB + 8));
-    if (W > share) W = share > 0 ? share : 1;
+    if (W > share) W = share;
     if (W > slots) W = slots;
     int best = 0x7fffffff;
     for (int w = W; w > W / 2; w--) {
@@ -979,8 +985,23 @@ Layout layout_with(int C, int W, int per_sm, int V, int size) {
     return L;
 }
 
+// Long rows have 13 warps in two blocks an SM, with two units of shared memory each; rows (or a block's part of them) of up to 18 units as many
+// warps as leave two units to a warp, in as many more blocks an SM, so that they stay in shared memory; rows of up to 4 units a warp a unit.
+// Policy loss with its gradient, us, in 2 / 3 / 5 / 6 / 10 blocks an SM: 4096 x 32000 bf16 146 / 124 / 126 / 126 / 135, 8192 x 50304 bf16
+// 357 / 433 / - / - / -, 16384 x 8000 bf16 296 / 228 / 165 / 165 / 168, 32768 x 2000 bf16 554 / 386 / 259 / 222 / 161.
+//
+// Where a row's units come a second time, out of L2, as many blocks share a row as keep what is in flight below 96 MB: 1 / 2 / 4 blocks a row took
+// 529 / 560 / 675 us for 4096 x 151936 bf16 (304 KB a row), 488 / 405 / 419 for 2072 x 128256 fp32 (513 KB), 519 / 495 / 413 for 1024 x 262144 fp32
+// (1 MB). Few rows are shared by as many blocks as there is room for: 4 x 32000 fp32 19.5 / 17.4 / 15.4, by eight 15.4.
+constexpr long long IN_FLIGHT = 96ll << 20;
 template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms) {
-    return layout_with(1, STATS ? 13 : 16, 2, V, (int)sizeof(T));
+    const int size = (int)sizeof(T), most = (int)(((long long)V * size + UB - 1) / UB);
+    int C = 1;
+    if (STATS && GRAD)
+        while (C < 8 && (most + C - 1) / C > 18 && 2ll * sms / C * most * UB > IN_FLIGHT) C *= 2;
+    while (C < 8 && 2ll * B * C <= 2ll * sms * 15 / 16 && most >= 8 * C) C *= 2;
+    const int share = (most + C - 1) / C, W = share <= 4 ? share : share <= 18 ? (share + 1) / 2 : 13, per_sm = 32 / (W + 1);
+    return layout_with(C, STATS || W < 13 ? W : 16, per_sm < 10 ? per_sm : 10, V, size);
 }
 
 template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(const LossArgs &a, cudaStream_t st) {
@@ -991,11 +1012,14 @@ template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(cons
     const size_t smem = smem_of(L);
     auto kernel = rows_kernel<T, STATS, GRAD, ENT>;
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     cfg.blockDim = dim3(32u * (unsigned int)(L.W + (STATS ? 1 : 0))); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned int)L.C; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.attrs = at; cfg.numAttrs = STATS && L.C > 1 ? 1 : 0;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    const bool clusters = STATS && L.C > 1;
+    cfg.attrs = at; cfg.numAttrs = clusters ? 1 : 0;
     // How many clusters the device holds at a time, asked once per device and layout: one too many would wait for all
     // rows of another (72 of four blocks, two an SM, fit where 74 would fill the SMs).
     static thread_local Fits known[MAX_DEVICES][4] = {};
@@ -1005,7 +1029,7 @@ template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(cons
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)block_smem(1));
         if (e != cudaSuccess) return e;
         fits = Fits{(int)cfg.blockDim.x, (int)smem, 0};
-        if (cfg.numAttrs) {
+        if (clusters) {
             cfg.gridDim = dim3((unsigned int)L.C);
             e = cudaOccupancyMaxActiveClusters(&fits.n, kernel, &cfg);
         } else {
@@ -1018,7 +1042,18 @@ template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(cons
     }
     L.rows_at_once = fits.n < a.B ? fits.n : a.B;
     cfg.gridDim = dim3((unsigned int)(L.rows_at_once * L.C));
+    if (a.follows) { cfg.attrs = clusters ? at : at + 1; cfg.numAttrs++; }
     return cudaLaunchKernelEx(&cfg, kernel, a, (const Layout)L);
+}
+
+// one block behind another kernel of the same call
+template <class... P> cudaError_t launch_one_block(void (*kernel)(P...), cudaStream_t st, P... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(1); cfg.blockDim = dim3(ST); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <bool STATS, bool GRAD> cudaError_t launch_type(const LossArgs &a, bool ent, cudaStream_t st) {
@@ -1040,11 +1075,9 @@ cudaError_t molla_loss_policy(const LossArgs &a, cudaStream_t st) {
     const bool ent = a.entropy != nullptr || a.entropy_coef != 0.0f;
     const cudaError_t e = a.grad ? launch_type<true, true>(a, ent, st) : launch_type<true, false>(a, ent, st);
     if (e != cudaSuccess) return e;
-    row_sum_kernel<<<1, ST, 0, st>>>(a.row_loss, a.B, a.scale, a.loss);
-    return cudaGetLastError();
+    return launch_one_block(row_sum_kernel, st, (const float *)a.row_loss, a.B, a.scale, a.loss);
 }
 
 cudaError_t molla_loss_pairs(const PairArgs &a, cudaStream_t st) {
-    pairs_kernel<<<1, ST, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch_one_block(pairs_kernel, st, a);
 }

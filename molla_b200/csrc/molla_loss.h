@@ -8,6 +8,7 @@
 struct LossArgs {
     const void *logits; int type; long long row_stride; int B, V;
     const int *tokens; const float *temperature;
+    bool follows;                // the launch is behind another one of the same call
     // outputs of a row (any but `logprob` and `status` may be nullptr)
     float *logprob; float *entropy; float *stats; unsigned int *status;
     // the gradient in the logits' type, or nullptr

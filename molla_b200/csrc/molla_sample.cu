@@ -2659,7 +2659,7 @@ int32_t molla_sample_preference_loss(const void *d_logits, int32_t logits_type, 
     p.loss = d_loss; p.pair_loss = d_pair_loss; p.margin = d_margin; p.seq_logratio = d_seq_logratio; p.pair_status = d_pair_status;
     p.g_logprob = d_grad_logits ? g : nullptr;
     if (e == cudaSuccess) e = molla_loss_pairs(p, (cudaStream_t)stream);
-    a.in_stats = stats; a.g_logprob = g;
+    a.in_stats = stats; a.g_logprob = g; a.follows = true;
     if (e == cudaSuccess && d_grad_logits) e = molla_loss_backward(a, (cudaStream_t)stream);
     return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "preference loss launch failed: %s", cudaGetErrorString(e));
 }

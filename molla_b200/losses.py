@@ -21,64 +21,72 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .sampler import _ptr, _stream_ptr
+from .sampler import _ptr
 
 _TYPES = {torch.float32: capi.LOGITS_FP32, torch.bfloat16: capi.LOGITS_BF16, torch.float16: capi.LOGITS_FP16}
+_F32, _I32 = torch.float32, torch.int32
 
 
 def _block(logits: torch.Tensor, tokens: torch.Tensor):
-    if logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda:
+    """(rows, vocabulary, row stride, type, pointers of logits and tokens, device index) of a block that can be read."""
+    kind = _TYPES.get(logits.dtype)
+    dev = logits.get_device()
+    if kind is None or dev < 0 or logits.dim() != 2:
         raise ValueError("logits must be a 2-D fp32, bf16 or fp16 CUDA tensor")
-    B, V = logits.shape
+    (B, V), (stride, step) = logits.shape, logits.stride()
     if V == 0:
         raise ValueError("logits need a vocabulary")
-    if B and (logits.stride(1) != 1 and V > 1 or logits.stride(0) < V and B > 1):
+    if B and (step != 1 and V > 1 or stride < V and B > 1):
         raise ValueError("logit rows must be contiguous and must not overlap")
-    _per_row("tokens", tokens, logits, B, torch.int32)
-    return B, V, max(logits.stride(0), V)
+    return B, V, stride if stride > V else V, kind, logits.data_ptr(), _values("tokens", tokens, dev, B, _I32), dev
 
 
-def _per_row(name: str, t, logits: torch.Tensor, n: int, dtype=torch.float32, what: str = "row"):
+def _values(name: str, t, dev: int, n: int, dtype=_F32, what: str = "row"):
+    """The pointer of a value a row, or None."""
     if t is None:
-        return
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (n,) or t.device != logits.device or not t.is_contiguous():
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != 1 or len(t) != n or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor of one value a {what} ({n}) on the logits' device")
+    return t.data_ptr()
 
 
 def _gradient(logits: torch.Tensor, stride: int, out):
-    """The gradient's tensor: the caller's, or a new one laid out like the logits."""
+    """The gradient's tensor (the caller's, or a new one laid out like the logits) and its row stride."""
     if out is None:
-        return torch.empty_strided(logits.shape, (stride, 1), dtype=logits.dtype, device=logits.device)
-    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or not out.is_cuda:
+        if logits.is_contiguous():
+            return torch.empty_like(logits), stride
+        return torch.empty_strided(logits.shape, (stride, 1), dtype=logits.dtype, device=logits.device), stride
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError("the gradient must have the logits' shape, type and device")
     if out.numel() and (out.stride(1) != 1 and out.shape[1] > 1 or out.stride(0) < out.shape[1] and out.shape[0] > 1):
         raise ValueError("gradient rows must be contiguous and must not overlap")
-    return out
+    return out, max(out.stride(0), out.shape[1])
 
 
-def _call(fn, logits: torch.Tensor, *args):
+def _call(fn, dev: int, *args):
     """A call of the library with the logits' device current."""
-    if logits.device.index == torch.cuda.current_device():
+    if dev == torch.cuda.current_device():
         rc = fn(*args)
     else:
-        with torch.cuda.device(logits.device):
+        with torch.cuda.device(dev):
             rc = fn(*args)
-    capi.check(rc)
+    if rc:
+        capi.check(rc)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature: torch.Tensor | None = None,
                    want_entropy: bool = False) -> dict:
     """Logprobs (and entropies) of one given token a row; token -1 is no token. `stats` is what
     `token_logprobs_backward` wants."""
-    B, V, stride = _block(logits, tokens)
-    _per_row("temperature", temperature, logits, B)
-    new = lambda *shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=logits.device)
-    out = dict(logprob=new(B), entropy=new(B) if want_entropy else None, stats=new(B, 2), row_status=new(B, dt=torch.int32))
+    B, V, stride, kind, x, tok, dev = _block(logits, tokens)
+    temp = _values("temperature", temperature, dev, B)
+    status = torch.empty_like(tokens)
+    stats = tokens.new_empty((B, 2), dtype=_F32)
+    logprob, entropy = stats.new_empty((2, B)).unbind(0) if want_entropy else (stats.new_empty(B), None)
     if B:
-        _call(capi.lib().molla_sample_token_logprobs, logits, _ptr(logits), _TYPES[logits.dtype], stride, B, V, _ptr(tokens),
-              _ptr(temperature), _stream_ptr(logits.device), _ptr(out["logprob"]), _ptr(out["entropy"]), _ptr(out["stats"]),
-              _ptr(out["row_status"]))
-    return out
+        _call(capi.lib().molla_sample_token_logprobs, dev, x, kind, stride, B, V, tok, temp, torch._C._cuda_getCurrentRawStream(dev),
+              logprob.data_ptr(), _ptr(entropy), stats.data_ptr(), status.data_ptr())
+    return dict(logprob=logprob, entropy=entropy, stats=stats, row_status=status)
 
 
 def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, scored: dict, grad_logprob: torch.Tensor,
@@ -86,22 +94,21 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, scored: 
                             out: torch.Tensor | None = None) -> torch.Tensor:
     """The logits' gradient of a loss with these derivatives by the rows' logprobs and entropies. `scored` is
     what `token_logprobs` returned for the same logits, tokens and temperatures. `out` may be the logits themselves."""
-    B, V, stride = _block(logits, tokens)
-    for name, t in (("temperature", temperature), ("grad_logprob", grad_logprob), ("grad_entropy", grad_entropy)):
-        _per_row(name, t, logits, B)
+    B, V, stride, kind, x, tok, dev = _block(logits, tokens)
+    temp = _values("temperature", temperature, dev, B)
+    g, h = _values("grad_logprob", grad_logprob, dev, B), _values("grad_entropy", grad_entropy, dev, B)
     if grad_logprob is None:
         raise ValueError("grad_logprob is required")
-    stats, entropy = scored["stats"], scored["entropy"] if grad_entropy is not None else None
-    if grad_entropy is not None and entropy is None:
+    stats, entropy = scored["stats"], scored["entropy"] if h is not None else None
+    if h is not None and entropy is None:
         raise ValueError("derivatives by the entropies need the entropies (want_entropy=True)")
-    if stats.shape != (B, 2) or stats.device != logits.device:
+    if stats.shape != (B, 2) or stats.get_device() != dev or stats.dtype != _F32 or not stats.is_contiguous():
         raise ValueError("the stats are of another block of logits")
-    _per_row("entropy", entropy, logits, B)
-    out = _gradient(logits, stride, out)
+    ent = _values("entropy", entropy, dev, B)
+    out, grad_stride = _gradient(logits, stride, out)
     if B:
-        _call(capi.lib().molla_sample_token_logprobs_backward, logits, _ptr(logits), _TYPES[logits.dtype], stride, B, V,
-              _ptr(tokens), _ptr(temperature), _ptr(stats), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy),
-              _stream_ptr(logits.device), _ptr(out), max(out.stride(0), V))
+        _call(capi.lib().molla_sample_token_logprobs_backward, dev, x, kind, stride, B, V, tok, temp, stats.data_ptr(), ent, g, h,
+              torch._C._cuda_getCurrentRawStream(dev), out.data_ptr(), grad_stride)
     return out
 
 
@@ -112,25 +119,25 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logprob: torch.T
                 want_grad: bool = True, want_entropy: bool = False, out: torch.Tensor | None = None) -> dict:
     """The clipped policy loss with a KL term and an entropy bonus, and the logits' gradient. Rows of weight 0 (prompts,
     padding) and of token -1 are not read. `out` (the gradient's place) may be the logits themselves."""
-    B, V, stride = _block(logits, tokens)
-    for name, t in (("old_logprob", old_logprob), ("advantage", advantage), ("weight", weight), ("ref_logprob", ref_logprob),
-                    ("temperature", temperature)):
-        _per_row(name, t, logits, B)
+    B, V, stride, kind, x, tok, dev = _block(logits, tokens)
     if old_logprob is None or advantage is None:
         raise ValueError("old logprobs and advantages are required")
-    grad = _gradient(logits, stride, out) if want_grad else None
-    new = lambda *shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=logits.device)
-    got = dict(loss=new(), row_loss=new(B), logprob=new(B), entropy=new(B) if want_entropy or entropy_coef != 0 else None,
-               kl=new(B) if ref_logprob is not None else None, clipped=new(B, dt=torch.bool), row_status=new(B, dt=torch.int32),
-               grad_logits=grad)
+    old, adv = _values("old_logprob", old_logprob, dev, B), _values("advantage", advantage, dev, B)
+    w, ref = _values("weight", weight, dev, B), _values("ref_logprob", ref_logprob, dev, B)
+    temp = _values("temperature", temperature, dev, B)
+    grad, grad_stride = _gradient(logits, stride, out) if want_grad else (None, 0)
+    # one tensor for what is a float a row (an allocation costs more than what the rest of this function does)
+    values = old_logprob.new_empty((2 + (ref is not None) + bool(want_entropy or entropy_coef), B)).unbind(0)
+    got = dict(loss=old_logprob.new_empty(()), row_loss=values[0], logprob=values[1],
+               entropy=values[-1] if want_entropy or entropy_coef else None, kl=values[2] if ref is not None else None,
+               clipped=old_logprob.new_empty(B, dtype=torch.bool), row_status=torch.empty_like(tokens), grad_logits=grad)
     if B == 0:
         got["loss"].zero_()
         return got
-    _call(capi.lib().molla_sample_policy_loss, logits, _ptr(logits), _TYPES[logits.dtype], stride, B, V, _ptr(tokens), _ptr(temperature),
-          _ptr(old_logprob), _ptr(advantage), _ptr(weight), _ptr(ref_logprob), clip_low, clip_high, kl_coef, entropy_coef, scale,
-          grad_scale, _stream_ptr(logits.device), _ptr(got["loss"]), _ptr(got["row_loss"]), _ptr(got["logprob"]),
-          _ptr(got["entropy"]), _ptr(got["kl"]), _ptr(got["clipped"]), _ptr(grad), max(grad.stride(0), V) if want_grad else 0,
-          _ptr(got["row_status"]))
+    _call(capi.lib().molla_sample_policy_loss, dev, x, kind, stride, B, V, tok, temp, old, adv, w, ref, clip_low, clip_high, kl_coef,
+          entropy_coef, scale, grad_scale, torch._C._cuda_getCurrentRawStream(dev), got["loss"].data_ptr(), got["row_loss"].data_ptr(),
+          got["logprob"].data_ptr(), _ptr(got["entropy"]), _ptr(got["kl"]), got["clipped"].data_ptr(), _ptr(grad), grad_stride,
+          got["row_status"].data_ptr())
     return got
 
 
@@ -141,28 +148,26 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, seq_off: torch.T
     """The preference loss over pairs of sequences, and the logits' gradient. `seq_off` (int32, 2 x pairs + 1, on the
     device) has the rows where the sequences begin and end, each pair's chosen one before its rejected one. `out` (the gradient's
     place) may be the logits themselves."""
-    B, V, stride = _block(logits, tokens)
-    if not isinstance(seq_off, torch.Tensor) or seq_off.dim() != 1 or seq_off.numel() % 2 != 1:
+    B, V, stride, kind, x, tok, dev = _block(logits, tokens)
+    if not isinstance(seq_off, torch.Tensor) or seq_off.dim() != 1 or len(seq_off) % 2 != 1:
         raise ValueError("seq_off must hold two sequences a pair and where the last one ends")
-    pairs = seq_off.numel() // 2
-    _per_row("seq_off", seq_off, logits, 2 * pairs + 1, torch.int32, "sequence")
-    _per_row("pair_weight", pair_weight, logits, pairs, what="pair")
-    for name, t in (("ref_logprob", ref_logprob), ("temperature", temperature)):
-        _per_row(name, t, logits, B)
-    grad = _gradient(logits, stride, out) if want_grad else None
-    new = lambda *shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=logits.device)
-    got = dict(loss=new(), pair_loss=new(pairs), margin=new(pairs), seq_logratio=new(2 * pairs), logprob=new(B),
-               row_status=new(B, dt=torch.int32), pair_status=new(pairs, dt=torch.int32), grad_logits=grad)
+    pairs = len(seq_off) // 2
+    off = _values("seq_off", seq_off, dev, 2 * pairs + 1, _I32, "sequence")
+    w, ref = _values("pair_weight", pair_weight, dev, pairs, what="pair"), _values("ref_logprob", ref_logprob, dev, B)
+    temp = _values("temperature", temperature, dev, B)
+    grad, grad_stride = _gradient(logits, stride, out) if want_grad else (None, 0)
+    of_pairs = seq_off.new_empty((4, pairs), dtype=_F32)
+    ratio, margin, loss = of_pairs[:2].view(-1), of_pairs[2], of_pairs[3]
+    got = dict(loss=of_pairs.new_empty(()), pair_loss=loss, margin=margin, seq_logratio=ratio, logprob=of_pairs.new_empty(B),
+               row_status=torch.empty_like(tokens), pair_status=seq_off.new_empty(pairs), grad_logits=grad)
     if B == 0:   # (the C entry point would be handed null pointers)
         if pairs:
             raise ValueError("pairs of sequences need rows")
         got["loss"].zero_()
         return got
     ws = capi.lib().molla_sample_preference_workspace_bytes(B)
-    buf = torch.empty(ws, dtype=torch.uint8, device=logits.device)
-    _call(capi.lib().molla_sample_preference_loss, logits, _ptr(logits), _TYPES[logits.dtype], stride, B, V, _ptr(tokens), _ptr(temperature),
-          _ptr(seq_off), pairs, _ptr(ref_logprob), _ptr(pair_weight), beta, label_smoothing, scale, grad_scale, _ptr(buf), ws,
-          _stream_ptr(logits.device), _ptr(got["loss"]), _ptr(got["pair_loss"]), _ptr(got["margin"]), _ptr(got["seq_logratio"]),
-          _ptr(got["logprob"]), _ptr(grad), max(grad.stride(0), V) if want_grad else 0, _ptr(got["row_status"]),
-          _ptr(got["pair_status"]))
+    buf = of_pairs.new_empty(ws // 4)
+    _call(capi.lib().molla_sample_preference_loss, dev, x, kind, stride, B, V, tok, temp, off, pairs, ref, w, beta, label_smoothing, scale,
+          grad_scale, buf.data_ptr(), ws, torch._C._cuda_getCurrentRawStream(dev), got["loss"].data_ptr(), loss.data_ptr(), margin.data_ptr(),
+          ratio.data_ptr(), got["logprob"].data_ptr(), _ptr(grad), grad_stride, got["row_status"].data_ptr(), got["pair_status"].data_ptr())
     return got
