@@ -124,10 +124,11 @@ __device__ __forceinline__ float exp_less_line(float q) {
 struct Answer { unsigned int status; Two l, lnS; float mean, ratio, q, kl; bool held; };
 
 template <bool ENT>
-__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in, float M, float S, float W, float c, Answer &o) {
-    o.status = in.status | (M == -INFINITY && S == 0.0f && !in.status ? MOLLA_ROW_EMPTY : 0u);
-    o.lnS = ln_of(S);
-    const float per_S = __frcp_rn(S);
+__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in, float M, Two S, float W, float c, Answer &o) {
+    o.status = in.status | (M == -INFINITY && S.hi == 0.0f && !in.status ? MOLLA_ROW_EMPTY : 0u);
+    const float per_S = __frcp_rn(S.hi);
+    o.lnS = ln_of(S.hi);
+    o.lnS.lo = __fmaf_rn(S.lo, per_S, o.lnS.lo);
     // ln p in the temperature that c stands for (log2(e)/T rounded): the error of c then moves ln S and the token together
     const float nats = c * LN2, nats_lo = __fadd_rn(__fmaf_rn(c, LN2, -nats), c * LN2_LEFT), dx = __fsub_rn(in.xt, M);
     o.mean = ENT ? W * per_S * nats : 0.0f;
@@ -325,7 +326,25 @@ __device__ __forceinline__ unsigned short lds2(uint32_t at) {
 template <> __device__ __forceinline__ float lds_element<__nv_bfloat16>(uint32_t at) { return __uint_as_float((unsigned int)lds2(at) << 16); }
 template <> __device__ __forceinline__ float lds_element<__half>(uint32_t at) { return __half2float(__ushort_as_half(lds2(at))); }
 
-struct Stat { float m, s, w; unsigned int late; };   // maximum, sum, weighted sum of a unit; a wait that ran out
+// maximum, sum (in two floats) and weighted sum of a unit; where a wait ran out s_lo is LATE
+struct Stat { float m, s, w, s_lo; };
+constexpr float LATE = -1.0f;
+
+// The sum over a warp of values from 0 to 64, to 2^-38 each: in integers of 2^-16 and, for what that leaves, of 2^-38 (the bits that an addition
+// to 192, or to 1.5 2^-15, ends in), which add up exactly in whatever order. (A tree of 32-bit sums loses what is below half a step of the
+// largest value, always downwards: 5e-8 of a unit, which the log ratio of a long sequence adds up.) A NaN stays.
+__device__ __forceinline__ Two warp_sum_exact(float v) {
+    const float high = __fadd_rn(v, 192.0f), left = __fsub_rn(v, __fsub_rn(high, 192.0f)), low = __fadd_rn(left, 1.5f / 32768.0f);
+    const int A = __reduce_add_sync(0xffffffffu, __float_as_int(high) - __float_as_int(192.0f));
+    const int B = __reduce_add_sync(0xffffffffu, __float_as_int(low) - __float_as_int(1.5f / 32768.0f));
+    const Two s = two_sum((float)(A >> 8) * (1.0f / 256.0f), __fmaf_rn((float)B, 1.0f / 274877906944.0f, (float)(A & 255) * (1.0f / 65536.0f)));
+    return __any_sync(0xffffffffu, !(v <= 64.0f)) ? Two{NAN, 0.0f} : s;
+}
+__device__ __forceinline__ void put_sum(Stat &o, float v) {
+    const Two s = warp_sum_exact(v);
+    o.s = s.hi;
+    o.s_lo = o.m == -INFINITY ? s.lo : __fmaf_rn(EX2_LOW, s.hi - 1.0f, s.lo);
+}
 
 // A unit's, from shared memory twice: once for its maximum, then for the sums (four of either a lane).
 template <class T, bool ENT, bool FULL>
@@ -341,7 +360,6 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
         }
     Stat o;
     o.m = warp_max(Chunk<T>::top(Chunk<T>::max(Chunk<T>::max(most.x, most.y), Chunk<T>::max(most.z, most.w))));
-    o.late = 0;
     const float m = o.m == -INFINITY ? 0.0f : o.m;   // nothing but -inf (and NaN): sums of 0 (and NaN)
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll(FULL ? KU / 2 : 1)
@@ -356,8 +374,7 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
                 if (ENT) w[i & 3] = __fmaf_rn(e, d < DEEP ? DEEP : d, w[i & 3]);
             }
         }
-    const float sum = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
-    o.s = o.m == -INFINITY ? sum : __fmaf_rn(EX2_LOW, sum - 1.0f, sum);
+    put_sum(o, (s[0] + s[1]) + (s[2] + s[3]));
     o.w = 0.0f;
     if (ENT) {
         const float ws = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
@@ -370,41 +387,48 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
 template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) {
     Stat o;
     o.m = warp_max(x);
-    o.late = 0;
-    const float m = o.m == -INFINITY ? 0.0f : o.m, d = __fsub_rn(x, m), e = ex2(d * c), sum = warp_sum(e);
-    o.s = o.m == -INFINITY ? sum : __fmaf_rn(EX2_LOW, sum - 1.0f, sum);
+    const float m = o.m == -INFINITY ? 0.0f : o.m, d = __fsub_rn(x, m), e = ex2(d * c);
+    put_sum(o, e);
     o.w = ENT ? warp_sum(e * (d < DEEP ? DEEP : d)) : 0.0f;
     return o;
 }
 
-// All units of a row: a warp, the units in turn over the lanes, then a tree.
-template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, float &S, float &W, unsigned int &late) {
+// All units of a row: a warp, the units in turn over the lanes, then a tree; S in two floats.
+template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, Two &S, float &W, bool &late) {
     const int lane = threadIdx.x & 31;
     constexpr int HELD = 3;   // units a lane that stay in registers
     Stat v[HELD];
     float m = -INFINITY;
-    unsigned int l = 0;
+    bool l = false;
 #pragma unroll
     for (int k = 0; k < HELD; k++) {
-        v[k] = Stat{-INFINITY, 0.0f, 0.0f, 0};
+        v[k] = Stat{-INFINITY, 0.0f, 0.0f, 0.0f};
         if (k * 32 + lane < n) v[k] = st[k * 32 + lane];
         m = fmaxf(m, v[k].m);
-        l |= v[k].late;
+        l |= v[k].s_lo == LATE;
     }
-    for (int u = HELD * 32 + lane; u < n; u += 32) { m = fmaxf(m, st[u].m); l |= st[u].late; }
+    for (int u = HELD * 32 + lane; u < n; u += 32) { m = fmaxf(m, st[u].m); l |= st[u].s_lo == LATE; }
     M = warp_max(m);
-    late = __any_sync(0xffffffffu, l != 0);
-    S = W = 0.0f;
+    late = __any_sync(0xffffffffu, l);
+    S = Two{0.0f, 0.0f};
+    W = 0.0f;
     const auto add = [&](const Stat &o) {
         const float d = o.m == -INFINITY ? 0.0f : __fsub_rn(o.m, M);   // (a unit of -inf: sums of 0, or NaN)
-        const float f = exp2_series(d * c);
-        S = __fmaf_rn(f, o.s, S);
+        const float f = exp2_series(d * c), p = f * o.s;
+        const Two s = two_sum(S.hi, p);
+        S = Two{s.hi, S.lo + (s.lo + __fmaf_rn(f, o.s_lo, __fmaf_rn(f, o.s, -p)))};
         if (ENT) W = __fmaf_rn(f, __fmaf_rn(d < DEEP ? DEEP : d, o.s, o.w), W);
     };
 #pragma unroll
     for (int k = 0; k < HELD; k++) add(v[k]);
     for (int u = HELD * 32 + lane; u < n; u += 32) add(st[u]);
-    S = warp_sum(S);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) {
+        const float hi = __shfl_xor_sync(0xffffffffu, S.hi, i), lo = __shfl_xor_sync(0xffffffffu, S.lo, i);
+        const Two s = two_sum(S.hi, hi);
+        S = Two{s.hi, (S.lo + lo) + s.lo};
+    }
+    S = two_sum(S.hi, S.lo);
     if (ENT) W = warp_sum(W);
 }
 
@@ -710,8 +734,9 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
         }
         if (!late) late = !wait_for(&ctl.sums[s], (n / DEPTH) & 1);
         if (GRAD && !alone) in.xt = st[L.table - 1].m;
-        float M, S, W;
-        unsigned int missed;
+        float M, W;
+        Two S;
+        bool missed;
         row_stat<ENT>(st, units, c, M, S, W, missed);
         late = late || missed;   // (what was lost once has the barriers out of step)
         if (late) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
@@ -726,7 +751,7 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
         } else if (lane < L.C) {   // nothing but the news that the table is free again
             put16(false, &ctl.share[s], lane, 0.0f, 0.0f, 0.0f, 0.0f, &ctl.answered[s]);
         }
-        if (first && lane == 0) row_write(a, r, in, M, S, o);
+        if (first && lane == 0) row_write(a, r, in, M, S.hi, o);
         n++;
     }
     if (late)   // what is still on its way to this block
@@ -795,15 +820,15 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
             for (int u = warp; u < span.units; u += warps) {
                 const uint32_t slot = feed.wait(held + units);
                 Stat o = u < span.full ? unit_stat<T, ENT, true>(slot, 0, c) : unit_stat<T, ENT, false>(slot, span.last_chunks(), c);
-                o.late = feed.late || LOSS_KNOB(a, 16);   // (testing build: a wait that ran out)
-                if (tell) put16(alone, st + u, lane, o.m, o.s, o.w, __uint_as_float(o.late), &ctl.sums[s]);
+                if (feed.late || LOSS_KNOB(a, 16)) o.s_lo = LATE;   // (testing build: a wait that ran out)
+                if (tell) put16(alone, st + u, lane, o.m, o.s, o.w, o.s_lo, &ctl.sums[s]);
                 if (GRAD && L.resident) units++;
                 else feed.give_back();
             }
             if (span.edge() && warp == span.units % warps) {
                 const int at = span.edge_at(lane);
                 const Stat o = edge_stat<ENT>(at != INT32_MIN ? to_f32(span.x[at]) : -INFINITY, c);
-                if (tell) put16(alone, st + span.units, lane, o.m, o.s, o.w, 0.0f, &ctl.sums[s]);
+                if (tell) put16(alone, st + span.units, lane, o.m, o.s, o.w, o.s_lo, &ctl.sums[s]);
             }
             // a warp without a unit says so: no row's answer may come before every warp is done with the rows before it
             __syncwarp();

@@ -45,7 +45,7 @@ def _values(name: str, t, dev: int, n: int, dtype=_F32, what: str = "row"):
     """The pointer of a value a row, or None."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != 1 or len(t) != n or t.get_device() != dev or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != (n,) or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor of one value a {what} ({n}) on the logits' device")
     return t.data_ptr()
 
@@ -126,11 +126,10 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logprob: torch.T
     w, ref = _values("weight", weight, dev, B), _values("ref_logprob", ref_logprob, dev, B)
     temp = _values("temperature", temperature, dev, B)
     grad, grad_stride = _gradient(logits, stride, out) if want_grad else (None, 0)
-    # one tensor for what is a float a row (an allocation costs more than what the rest of this function does)
-    values = old_logprob.new_empty((2 + (ref is not None) + bool(want_entropy or entropy_coef), B)).unbind(0)
-    got = dict(loss=old_logprob.new_empty(()), row_loss=values[0], logprob=values[1],
-               entropy=values[-1] if want_entropy or entropy_coef else None, kl=values[2] if ref is not None else None,
-               clipped=old_logprob.new_empty(B, dtype=torch.bool), row_status=torch.empty_like(tokens), grad_logits=grad)
+    new = torch.empty_like   # (of the allocations PyTorch has the cheapest)
+    got = dict(loss=old_logprob.new_empty(()), row_loss=new(old_logprob), logprob=new(old_logprob),
+               entropy=new(old_logprob) if want_entropy or entropy_coef else None, kl=new(old_logprob) if ref is not None else None,
+               clipped=new(old_logprob, dtype=torch.bool), row_status=new(tokens), grad_logits=grad)
     if B == 0:
         got["loss"].zero_()
         return got
@@ -156,18 +155,17 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, seq_off: torch.T
     w, ref = _values("pair_weight", pair_weight, dev, pairs, what="pair"), _values("ref_logprob", ref_logprob, dev, B)
     temp = _values("temperature", temperature, dev, B)
     grad, grad_stride = _gradient(logits, stride, out) if want_grad else (None, 0)
-    of_pairs = seq_off.new_empty((4, pairs), dtype=_F32)
-    ratio, margin, loss = of_pairs[:2].view(-1), of_pairs[2], of_pairs[3]
-    got = dict(loss=of_pairs.new_empty(()), pair_loss=loss, margin=margin, seq_logratio=ratio, logprob=of_pairs.new_empty(B),
-               row_status=torch.empty_like(tokens), pair_status=seq_off.new_empty(pairs), grad_logits=grad)
+    new = tokens.new_empty
+    got = dict(loss=new((), dtype=_F32), pair_loss=new(pairs, dtype=_F32), margin=new(pairs, dtype=_F32), seq_logratio=new(2 * pairs, dtype=_F32),
+               logprob=new(B, dtype=_F32), row_status=new(B), pair_status=new(pairs), grad_logits=grad)
     if B == 0:   # (the C entry point would be handed null pointers)
         if pairs:
             raise ValueError("pairs of sequences need rows")
         got["loss"].zero_()
         return got
     ws = capi.lib().molla_sample_preference_workspace_bytes(B)
-    buf = of_pairs.new_empty(ws // 4)
+    buf = new(ws // 4)
     _call(capi.lib().molla_sample_preference_loss, dev, x, kind, stride, B, V, tok, temp, off, pairs, ref, w, beta, label_smoothing, scale,
-          grad_scale, buf.data_ptr(), ws, torch._C._cuda_getCurrentRawStream(dev), got["loss"].data_ptr(), loss.data_ptr(), margin.data_ptr(),
-          ratio.data_ptr(), got["logprob"].data_ptr(), _ptr(grad), grad_stride, got["row_status"].data_ptr(), got["pair_status"].data_ptr())
+          grad_scale, buf.data_ptr(), ws, torch._C._cuda_getCurrentRawStream(dev), got["loss"].data_ptr(), got["pair_loss"].data_ptr(),
+          got["margin"].data_ptr(), got["seq_logratio"].data_ptr(), got["logprob"].data_ptr(), _ptr(grad), grad_stride, got["row_status"].data_ptr(), got["pair_status"].data_ptr())
     return got
