@@ -349,6 +349,10 @@ __device__ __forceinline__ void put_sum(Stat &o, float v) {
 // A unit's, from shared memory twice: once for its maximum, then for the sums (four of either a lane).
 template <class T, bool ENT, bool FULL>
 __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
+    // What rounding c (x - m) leaves out comes back into the sum for logits of 32 bits: a logprob is off by 2e-8 in place of 6e-8, at two more
+    // operations a logit, which memory hides (2072 x 128256 407 us with it, 405 without). For 16 bits, rounded to 2^-9 themselves, it
+    // does not (4096 x 151936 557 and 531, scores of 4144 x 128256 233 and 213).
+    constexpr bool SHARP = sizeof(T) == 4;
     const int lane = threadIdx.x & 31;
     constexpr unsigned int low = Chunk<T>::LOWEST;
     uint4 most = make_uint4(low, low, low, low);
@@ -361,7 +365,7 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
     Stat o;
     o.m = warp_max(Chunk<T>::top(Chunk<T>::max(Chunk<T>::max(most.x, most.y), Chunk<T>::max(most.z, most.w))));
     const float m = o.m == -INFINITY ? 0.0f : o.m;   // nothing but -inf (and NaN): sums of 0 (and NaN)
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, w[4] = {0.0f, 0.0f, 0.0f, 0.0f}, left[2] = {0.0f, 0.0f};
 #pragma unroll(FULL ? KU / 2 : 1)
     for (int k = 0; k < KU; k++)
         if (FULL || k * 32 + lane < chunks) {
@@ -369,12 +373,16 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
             Chunk<T>::get(lds16(slot + k * 512 + lane * 16), x);
 #pragma unroll
             for (int i = 0; i < Chunk<T>::N; i++) {
-                const float d = __fsub_rn(x[i], m), e = ex2(d * c);
+                float d = __fsub_rn(x[i], m);
+                if (SHARP || ENT) d = d < DEEP ? DEEP : d;
+                const float t = d * c, e = ex2(t);
                 s[i & 3] += e;
-                if (ENT) w[i & 3] = __fmaf_rn(e, d < DEEP ? DEEP : d, w[i & 3]);
+                if (SHARP) left[i & 1] = __fmaf_rn(e, __fmaf_rn(d, c, -t), left[i & 1]);
+                if (ENT) w[i & 3] = __fmaf_rn(e, d, w[i & 3]);
             }
         }
     put_sum(o, (s[0] + s[1]) + (s[2] + s[3]));
+    if (SHARP) o.s_lo = __fmaf_rn(warp_sum(left[0] + left[1]), LN2, o.s_lo);
     o.w = 0.0f;
     if (ENT) {
         const float ws = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
@@ -559,6 +567,8 @@ template <class T, bool STATS, bool GRAD> struct Feed {
         while (more && ahead < L.R) fetch();
     }
     __device__ __forceinline__ bool row_ok(int k) const { return (long long)row0 + (long long)k * step < a.B; }
+    // A gradient that follows another pass over the logits takes the rows from the last to the first: those are still in L2.
+    __device__ __forceinline__ int row_of(int k) const { return !STATS && a.follows ? a.B - 1 - (row0 + k * step) : row0 + k * step; }
     __device__ __forceinline__ void start(int r) {
         const RowSpan<T> span((const T *)a.logits + (long long)r * a.row_stride, a.V);
         src = (const char *)span.x + warp * UB;
@@ -572,9 +582,9 @@ template <class T, bool STATS, bool GRAD> struct Feed {
             if (i - base >= 32) {
                 base = i;
                 const int lane = threadIdx.x & 31;
-                mask = __ballot_sync(0xffffffffu, row_ok(i + lane) && row_read<STATS>(a, row0 + (i + lane) * step));
+                mask = __ballot_sync(0xffffffffu, row_ok(i + lane) && row_read<STATS>(a, row_of(i + lane)));
             }
-            if (mask >> (i - base) & 1) return row0 + i * step;
+            if (mask >> (i - base) & 1) return row_of(i);
         }
     }
     // From the end of one row's units to the first of another: a row for its sums, then, where units do not stay (see rows_kernel), the row before
@@ -794,14 +804,14 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
     int held = 0;         // units that stay for the gradient of the row before
     int before = -1;      // that row
     for (int i = 0;; i++) {
-        const int r = row0 + i * step, from = i % 32;
+        const int r = feed.row_of(i), from = i % 32;
         const bool last = !feed.row_ok(i);
         if (last && before < 0) break;
         if (from == 0 && !last) {
-            const bool ok = feed.row_ok(i + lane), read = ok && row_read<STATS>(a, row0 + (i + lane) * step);
+            const bool ok = feed.row_ok(i + lane), read = ok && row_read<STATS>(a, feed.row_of(i + lane));
             mask = __ballot_sync(0xffffffffu, read);
-            if (!STATS && read) mine = row_given(a, row0 + (i + lane) * step);
-            if (STATS) mine.c = LOG2E / (read && a.temperature ? a.temperature[row0 + (i + lane) * step] : 1.0f);
+            if (!STATS && read) mine = row_given(a, feed.row_of(i + lane));
+            if (STATS) mine.c = LOG2E / (read && a.temperature ? a.temperature[feed.row_of(i + lane)] : 1.0f);
         }
         if (!last && !(mask >> from & 1)) {
             if (GRAD) zero_row<T>((T *)a.grad + (long long)r * a.grad_stride, a.V, warp, warps);
@@ -909,11 +919,11 @@ __global__ void __launch_bounds__(ST) row_sum_kernel(const float *row_loss, int 
     if (threadIdx.x == 0) *loss = (float)(v * (double)scale);
 }
 
-// A warp adds up the log ratios of a sequence's rows, each lane every 32nd, then the lanes in the order of a tree.
-__device__ double sequence_sum(const PairArgs &a, int from, int to, unsigned int *status) {
-    const int lane = threadIdx.x & 31;
+// Warps adds up the log ratios of a sequence's rows: each lane every so-manieth, then the lanes in the order of a tree.
+__device__ double sequence_sum(const PairArgs &a, int from, int to, int step, unsigned int *status) {
     double v = 0.0;
-    for (int r = from + lane; r < to; r += 32) {
+#pragma unroll 4
+    for (int r = from; r < to; r += step) {
         *status |= a.row_status[r] & ROW_ERRORS;
         if (a.tokens[r] != -1) v += (double)a.logprob[r] - (a.ref_logprob ? (double)a.ref_logprob[r] : 0.0);
     }
@@ -926,9 +936,10 @@ __device__ double sequence_sum(const PairArgs &a, int from, int to, unsigned int
 __device__ __forceinline__ double soft(double m) { return fmax(m, 0.0) + log1p(exp(-fabs(m))); }
 __device__ __forceinline__ double sigmoid(double m) { return m >= 0.0 ? 1.0 / (1.0 + exp(-m)) : exp(m) / (1.0 + exp(m)); }
 
-// One block: the pairs a warp each, in turn.
+// One block: the pairs a warp each, or, if they are few, as many warps as there are for each.
 __global__ void __launch_bounds__(ST) pairs_kernel(const __grid_constant__ PairArgs a) {
-    __shared__ double ws[ST / 32];
+    __shared__ double ws[ST / 32], chosen[ST / 32], rejected[ST / 32];
+    __shared__ unsigned int statuses[ST / 32];
     wait_for_launch_before();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, S = 2 * a.n_pairs;
     int bad = 0;
@@ -939,10 +950,23 @@ __global__ void __launch_bounds__(ST) pairs_kernel(const __grid_constant__ PairA
         for (int r = threadIdx.x; r < first; r += ST) a.g_logprob[r] = 0.0f;
         for (int r = last + threadIdx.x; r < a.B; r += ST) a.g_logprob[r] = 0.0f;
     }
+    int at_once = 1;   // pairs, of `each` warps
+    while (at_once < a.n_pairs && at_once < ST / 32) at_once *= 2;
+    const int each = ST / 32 / at_once, group = warp / each, of_pair = threadIdx.x - group * each * 32, step = each * 32;
     double total = 0.0;
-    for (int p = warp; p < a.n_pairs; p += ST / 32) {
+    for (int p0 = 0; p0 < a.n_pairs; p0 += at_once) {
+        const int p = p0 + group;
+        const bool mine = p < a.n_pairs && !broken;
+        const int o0 = mine ? a.off[2 * p] : 0, o1 = mine ? a.off[2 * p + 1] : 0, o2 = mine ? a.off[2 * p + 2] : 0;
+        unsigned int status = 0;
+        const double c = sequence_sum(a, o0 + of_pair, o1, step, &status), d = sequence_sum(a, o1 + of_pair, o2, step, &status);
+        status = __reduce_or_sync(0xffffffffu, status);
+        __syncthreads();
+        if (lane == 0) { chosen[warp] = c; rejected[warp] = d; statuses[warp] = status; }
+        __syncthreads();
+        if (p >= a.n_pairs) continue;
         if (broken) {
-            if (lane == 0) {
+            if (of_pair == 0) {
                 const int *o = a.off + 2 * p;
                 a.pair_status[p] = o[0] < 0 || o[1] < o[0] || o[2] < o[1] || o[2] > a.B ? MOLLA_ROW_INVALID_CONFIG : 0u;
                 a.pair_loss[p] = a.margin[p] = a.seq_logratio[2 * p] = a.seq_logratio[2 * p + 1] = NAN;
@@ -950,23 +974,22 @@ __global__ void __launch_bounds__(ST) pairs_kernel(const __grid_constant__ PairA
             total = NAN;
             continue;
         }
-        const int o0 = a.off[2 * p], o1 = a.off[2 * p + 1], o2 = a.off[2 * p + 2];
-        unsigned int status = 0;
-        const double sc = sequence_sum(a, o0, o1, &status), sr = sequence_sum(a, o1, o2, &status);
-        status = __reduce_or_sync(0xffffffffu, status);
+        double sc = 0.0, sr = 0.0;
+        status = 0;
+        for (int k = group * each; k < (group + 1) * each; k++) { sc += chosen[k]; sr += rejected[k]; status |= statuses[k]; }
         const double beta = a.beta, eps = a.smoothing, w = a.weight ? (double)a.weight[p] : 1.0, m = beta * (sc - sr);
         const double l = w == 0.0 ? 0.0 : w * ((1.0 - eps) * soft(-m) + eps * soft(m));
         const double dm = status || w == 0.0 ? 0.0 : w * (eps * sigmoid(m) - (1.0 - eps) * sigmoid(-m));
-        total += l;
-        if (lane == 0) {
+        if (of_pair == 0) {
+            total += l;
             a.pair_status[p] = status;
             a.pair_loss[p] = (float)l; a.margin[p] = (float)m;
             a.seq_logratio[2 * p] = (float)sc; a.seq_logratio[2 * p + 1] = (float)sr;
         }
         if (a.g_logprob) {
             const float g = (float)(beta * dm * (double)a.scale * (double)a.grad_scale);
-            for (int r = o0 + lane; r < o1; r += 32) a.g_logprob[r] = g;
-            for (int r = o1 + lane; r < o2; r += 32) a.g_logprob[r] = -g;
+            for (int r = o0 + of_pair; r < o1; r += step) a.g_logprob[r] = g;
+            for (int r = o1 + of_pair; r < o2; r += step) a.g_logprob[r] = -g;
         }
     }
     total = sum_1024(lane == 0 ? total : 0.0, ws);
