@@ -27,7 +27,7 @@ using namespace molla;
 namespace {
 
 constexpr double LOG2E_64 = 1.44269504088896340736;
-constexpr float LOG2E = (float)LOG2E_64;
+constexpr float LOG2E = (float)LOG2E_64, LOG2E_LEFT = (float)(LOG2E_64 - (double)LOG2E);
 constexpr float DEEP = -1e30f;    // where x - M is held, so that 0 * (x - M) is 0 for logits of -inf too
 constexpr unsigned int ROW_ERRORS = MOLLA_ROW_BAD_TOKEN | MOLLA_ROW_EMPTY | MOLLA_ROW_INVALID_CONFIG | MOLLA_ROW_LOAD_TIMEOUT;
 
@@ -96,7 +96,7 @@ __device__ __forceinline__ Two two_sum(float a, float b) {
 }
 __device__ __forceinline__ bool ordinary(float x) { return fabsf(x) < 3e38f; }
 
-constexpr float LN2 = 0.693147180559945309f, LN2_LEFT = (float)(0.693147180559945309 - (double)LN2);
+constexpr float LN2 = 0.693147180559945309f;
 constexpr float LN2_SHORT = 0.693145751953125f, LN2_REST = (float)(0.693147180559945309 - 0.693145751953125);   // 17 bits, times a small integer exact
 
 // ln S, S > 0: the power of two apart; what is left lies within a factor of the square root of two of one, its logarithm is below 0.35 and
@@ -124,13 +124,17 @@ __device__ __forceinline__ float exp_less_line(float q) {
 struct Answer { unsigned int status; Two l, lnS; float mean, ratio, q, kl; bool held; };
 
 template <bool ENT>
-__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in, float M, Two S, float W, float c, Answer &o) {
+__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in, float M, Two S, float W, float depth, float c, Answer &o) {
     o.status = in.status | (M == -INFINITY && S.hi == 0.0f && !in.status ? MOLLA_ROW_EMPTY : 0u);
     const float per_S = __frcp_rn(S.hi);
     o.lnS = ln_of(S.hi);
     o.lnS.lo = __fmaf_rn(S.lo, per_S, o.lnS.lo);
-    // ln p in the temperature that c stands for (log2(e)/T rounded): the error of c then moves ln S and the token together
-    const float nats = c * LN2, nats_lo = __fadd_rn(__fmaf_rn(c, LN2, -nats), c * LN2_LEFT), dx = __fsub_rn(in.xt, M);
+    // c is log2(e)/T rounded, off by a part `off` of up to 2^-24, and with it ln S by off times the mean depth: of a logprob an error of 4e-8 at T = 1,
+    // always to the same side. An estimate of the depth that is right to a third takes it out (the logprobs' mean and standard error against 64
+    // bits before, over 128256 logits: 2e-8 and 5.5e-8).
+    const float off = (__fmaf_rn(c, in.T, -LOG2E) - LOG2E_LEFT) * LN2;
+    o.lnS.lo = __fmaf_rn(off, depth, o.lnS.lo);
+    const float nats = in.per_T, nats_lo = __fmaf_rn(-in.T, nats, 1.0f) * nats, dx = __fsub_rn(in.xt, M);
     o.mean = ENT ? W * per_S * nats : 0.0f;
     if (ordinary(dx) && ordinary(o.lnS.hi)) {
         const Two d = two_sum(in.xt, -M);
@@ -160,6 +164,7 @@ __device__ __forceinline__ void row_write(const LossArgs &a, int r, const RowIn 
     const double H = ((double)o.lnS.hi + (double)o.lnS.lo) - (double)o.mean;
     a.status[r] = status;
     a.logprob[r] = status ? NAN : o.l.hi;
+    if (a.logprob_lo) a.logprob_lo[r] = status ? 0.0f : o.l.lo;
     if (a.entropy) a.entropy[r] = status ? NAN : (float)H;
     if (a.stats) { a.stats[2 * r] = status ? NAN : M; a.stats[2 * r + 1] = status ? 0.0f : S; }
     if (!a.row_loss) return;
@@ -182,6 +187,7 @@ __device__ __forceinline__ void row_refused(const LossArgs &a, int r, const RowI
 __device__ void row_idle(const LossArgs &a, int r) {
     a.status[r] = 0;
     a.logprob[r] = 0.0f;
+    if (a.logprob_lo) a.logprob_lo[r] = 0.0f;
     if (a.entropy) a.entropy[r] = 0.0f;
     if (a.stats) { a.stats[2 * r] = 0.0f; a.stats[2 * r + 1] = 1.0f; }
     if (a.row_loss) a.row_loss[r] = 0.0f;
@@ -349,10 +355,6 @@ __device__ __forceinline__ void put_sum(Stat &o, float v) {
 // A unit's, from shared memory twice: once for its maximum, then for the sums (four of either a lane).
 template <class T, bool ENT, bool FULL>
 __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
-    // What rounding c (x - m) leaves out comes back into the sum for logits of 32 bits: a logprob is off by 2e-8 in place of 6e-8, at two more
-    // operations a logit, which memory hides (2072 x 128256 407 us with it, 405 without). For 16 bits, rounded to 2^-9 themselves, it
-    // does not (4096 x 151936 557 and 531, scores of 4144 x 128256 233 and 213).
-    constexpr bool SHARP = sizeof(T) == 4;
     const int lane = threadIdx.x & 31;
     constexpr unsigned int low = Chunk<T>::LOWEST;
     uint4 most = make_uint4(low, low, low, low);
@@ -365,7 +367,7 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
     Stat o;
     o.m = warp_max(Chunk<T>::top(Chunk<T>::max(Chunk<T>::max(most.x, most.y), Chunk<T>::max(most.z, most.w))));
     const float m = o.m == -INFINITY ? 0.0f : o.m;   // nothing but -inf (and NaN): sums of 0 (and NaN)
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, w[4] = {0.0f, 0.0f, 0.0f, 0.0f}, left[2] = {0.0f, 0.0f};
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll(FULL ? KU / 2 : 1)
     for (int k = 0; k < KU; k++)
         if (FULL || k * 32 + lane < chunks) {
@@ -373,16 +375,12 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
             Chunk<T>::get(lds16(slot + k * 512 + lane * 16), x);
 #pragma unroll
             for (int i = 0; i < Chunk<T>::N; i++) {
-                float d = __fsub_rn(x[i], m);
-                if (SHARP || ENT) d = d < DEEP ? DEEP : d;
-                const float t = d * c, e = ex2(t);
+                const float d = __fsub_rn(x[i], m), e = ex2(d * c);
                 s[i & 3] += e;
-                if (SHARP) left[i & 1] = __fmaf_rn(e, __fmaf_rn(d, c, -t), left[i & 1]);
-                if (ENT) w[i & 3] = __fmaf_rn(e, d, w[i & 3]);
+                if (ENT) w[i & 3] = __fmaf_rn(e, d < DEEP ? DEEP : d, w[i & 3]);
             }
         }
     put_sum(o, (s[0] + s[1]) + (s[2] + s[3]));
-    if (SHARP) o.s_lo = __fmaf_rn(warp_sum(left[0] + left[1]), LN2, o.s_lo);
     o.w = 0.0f;
     if (ENT) {
         const float ws = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
@@ -401,8 +399,9 @@ template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) 
     return o;
 }
 
-// All units of a row: a warp, the units in turn over the lanes, then a tree; S in two floats.
-template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, Two &S, float &W, bool &late) {
+// All units of a row: a warp, the units in turn over the lanes, then a tree; S in two floats. `depth`: about how far in nats the logits are
+// below M on the average of the distribution; within a unit, what is not its maximum is taken to be 2.5 below it (see row_answer).
+template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, Two &S, float &W, float &depth, bool &late) {
     const int lane = threadIdx.x & 31;
     constexpr int HELD = 3;   // units a lane that stay in registers
     Stat v[HELD];
@@ -419,11 +418,12 @@ template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int
     M = warp_max(m);
     late = __any_sync(0xffffffffu, l);
     S = Two{0.0f, 0.0f};
-    W = 0.0f;
+    W = depth = 0.0f;
     const auto add = [&](const Stat &o) {
         const float d = o.m == -INFINITY ? 0.0f : __fsub_rn(o.m, M);   // (a unit of -inf: sums of 0, or NaN)
-        const float f = exp2_series(d * c), p = f * o.s;
+        const float t = d * c, f = exp2_series(t), p = f * o.s;
         const Two s = two_sum(S.hi, p);
+        depth = __fmaf_rn(f, __fmaf_rn(t < DEEP ? -DEEP : -t, LN2 * o.s, 2.5f * fmaxf(o.s - 1.0f, 0.0f)), depth);
         S = Two{s.hi, S.lo + (s.lo + __fmaf_rn(f, o.s_lo, __fmaf_rn(f, o.s, -p)))};
         if (ENT) W = __fmaf_rn(f, __fmaf_rn(d < DEEP ? DEEP : d, o.s, o.w), W);
     };
@@ -435,8 +435,10 @@ template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int
         const float hi = __shfl_xor_sync(0xffffffffu, S.hi, i), lo = __shfl_xor_sync(0xffffffffu, S.lo, i);
         const Two s = two_sum(S.hi, hi);
         S = Two{s.hi, (S.lo + lo) + s.lo};
+        depth += __shfl_xor_sync(0xffffffffu, depth, i);
     }
     S = two_sum(S.hi, S.lo);
+    depth *= __frcp_rn(S.hi);
     if (ENT) W = warp_sum(W);
 }
 
@@ -744,14 +746,14 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
         }
         if (!late) late = !wait_for(&ctl.sums[s], (n / DEPTH) & 1);
         if (GRAD && !alone) in.xt = st[L.table - 1].m;
-        float M, W;
+        float M, W, depth;
         Two S;
         bool missed;
-        row_stat<ENT>(st, units, c, M, S, W, missed);
+        row_stat<ENT>(st, units, c, M, S, W, depth, missed);
         late = late || missed;   // (what was lost once has the barriers out of step)
         if (late) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
         Answer o;
-        const RowGrad q = row_answer<ENT>(a, in, M, S, W, c, o);
+        const RowGrad q = row_answer<ENT>(a, in, M, S, W, depth, c, o);
         __syncwarp();
         if (GRAD || alone) {
             if (lane == 0) {
@@ -925,7 +927,7 @@ __device__ double sequence_sum(const PairArgs &a, int from, int to, int step, un
 #pragma unroll 4
     for (int r = from; r < to; r += step) {
         *status |= a.row_status[r] & ROW_ERRORS;
-        if (a.tokens[r] != -1) v += (double)a.logprob[r] - (a.ref_logprob ? (double)a.ref_logprob[r] : 0.0);
+        if (a.tokens[r] != -1) v += ((double)a.logprob[r] - (a.ref_logprob ? (double)a.ref_logprob[r] : 0.0)) + (double)a.logprob_lo[r];
     }
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) v += __shfl_xor_sync(0xffffffffu, v, i);
@@ -1010,21 +1012,27 @@ int sm_count_of(int &dev) {
 
 constexpr size_t block_smem(int per_sm) { return (size_t)(228 / per_sm - 2) * 1024; }   // of a block's dynamic shared memory: an SM's 228 KB less what each block takes besides
 
-// C blocks a row, W warps a block or as many fewer as share its units evenly (6 % of the rounds idle), and the shared memory of
-// `per_sm` blocks an SM.
+// W warps, or as many fewer as share a block's units evenly (6 % of the rounds idle).
+int even(int share, int W) {
+    int best = 0x7fffffff, chosen = 1;
+    if (W > share) W = share;
+    for (int w = W; w > W / 2; w--) {
+        const int rounds = (share + w - 1) / w * w;
+        if (rounds < best && (best == 0x7fffffff || best * 16 > share * 17)) { best = rounds; chosen = w; }
+    }
+    return chosen;
+}
+
+// C blocks a row, at most W warps a block, and the shared memory of `per_sm` blocks an SM.
 Layout layout_with(int C, int W, int per_sm, int V, int size) {
     Layout L{};
     const int unit = UB / size, most = (int)(((long long)V * size + UB - 1) / UB), share = (most + C - 1) / C;   // units of a row, and of a block
     L.C = C;
     L.table = max((V + unit - 1) / unit + 1, C * W) + 1;   // (an unaligned row's whole chunks and its edge, or a place a warp; the token's logit)
-    const int slots = (int)((block_smem(per_sm) - DEPTH * (size_t)L.table * sizeof(Stat)) / (UB + 8));
-    if (W > share) W = share;
-    if (W > slots) W = slots;
-    int best = 0x7fffffff;
-    for (int w = W; w > W / 2; w--) {
-        const int rounds = (share + w - 1) / w * w;
-        if (rounds < best && (best == 0x7fffffff || best * 16 > share * 17)) { best = rounds; L.W = w; }
-    }
+    const auto room = [&] { const size_t all = block_smem(per_sm), tables = DEPTH * (size_t)L.table * sizeof(Stat); return all > tables ? (int)((all - tables) / (UB + 8)) : 0; };
+    while (per_sm > 1 && room() < (W < share ? W : share)) per_sm--;   // (the widest rows' tables)
+    const int slots = room();
+    L.W = even(share, W < slots ? W : slots);
     const int each = (share + L.W - 1) / L.W;
     L.R = slots / L.W;
     if (L.R > 32) L.R = 32;
@@ -1038,6 +1046,9 @@ Layout layout_with(int C, int W, int per_sm, int V, int size) {
 // Policy loss with its gradient, us, in 2 / 3 / 5 / 6 / 10 blocks an SM: 4096 x 32000 bf16 146 / 124 / 126 / 126 / 135, 8192 x 50304 bf16
 // 357 / 433 / - / - / -, 16384 x 8000 bf16 296 / 228 / 165 / 165 / 168, 32768 x 2000 bf16 554 / 386 / 259 / 222 / 161.
 //
+// Without a gradient nothing waits for an answer, and more blocks of fewer warps are better: 13 warps in two blocks an SM, 7 in four, us: 2048 x 128256 bf16
+// 123 / 111, 8288 x 128256 bf16 395 / 381, 4096 x 128256 fp32 350 / 339.
+//
 // Where a row's units come a second time, out of L2, as many blocks share a row as keep what is in flight below 96 MB: 1 / 2 / 4 blocks a row took
 // 529 / 560 / 675 us for 4096 x 151936 bf16 (304 KB a row), 488 / 405 / 419 for 2072 x 128256 fp32 (513 KB), 519 / 495 / 413 for 1024 x 262144 fp32
 // (1 MB). Few rows are shared by as many blocks as there is room for: 4 x 32000 fp32 19.5 / 17.4 / 15.4, by eight 15.4.
@@ -1048,8 +1059,12 @@ template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms
     if (STATS && GRAD)
         while (C < 8 && (most + C - 1) / C > 18 && 2ll * sms / C * most * UB > IN_FLIGHT) C *= 2;
     while (C < 8 && 2ll * B * C <= 2ll * sms * 15 / 16 && most >= 8 * C) C *= 2;
-    const int share = (most + C - 1) / C, W = share <= 4 ? share : share <= 18 ? (share + 1) / 2 : 13, per_sm = 32 / (W + 1);
-    return layout_with(C, STATS || W < 13 ? W : 16, per_sm < 10 ? per_sm : 10, V, size);
+    const int share = (most + C - 1) / C;
+    int W = share <= 4 ? share : share <= 18 ? (share + 1) / 2 : STATS ? 13 : 16;
+    if (STATS && !GRAD && (long long)B * C > sms) W = even(share, share <= 6 ? (share + 1) / 2 : 7);
+    else if (W < 13) W = even(share, W);
+    const int per_sm = W >= 13 ? 2 : 32 / (W + 1);
+    return layout_with(C, W, per_sm < 10 ? per_sm : 10, V, size);
 }
 
 template <class T, bool STATS, bool GRAD, bool ENT> cudaError_t launch_rows(const LossArgs &a, cudaStream_t st) {

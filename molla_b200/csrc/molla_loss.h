@@ -10,7 +10,7 @@ struct LossArgs {
     const int *tokens; const float *temperature;
     bool follows;                // the launch is behind another one of the same call
     // outputs of a row (any but `logprob` and `status` may be nullptr)
-    float *logprob; float *entropy; float *stats; unsigned int *status;
+    float *logprob; float *logprob_lo; float *entropy; float *stats; unsigned int *status;   // logprob_lo: what the logprob's rounding leaves out
     // the gradient in the logits' type, or nullptr
     void *grad; long long grad_stride;
     // the row's derivatives, where they are given: by logprob (nullptr = the policy loss has them) and by entropy
@@ -27,7 +27,7 @@ struct LossArgs {
 // The preference loss between its two passes over the logits.
 struct PairArgs {
     int B, n_pairs;
-    const int *tokens; const int *off; const float *logprob; const float *ref_logprob; const float *weight; const unsigned int *row_status;
+    const int *tokens; const int *off; const float *logprob; const float *logprob_lo; const float *ref_logprob; const float *weight; const unsigned int *row_status;
     float beta, smoothing, scale, grad_scale;
     float *loss; float *pair_loss; float *margin; float *seq_logratio; unsigned int *pair_status;
     float *g_logprob;            // [B] the rows' derivatives, or nullptr

@@ -2622,7 +2622,7 @@ int32_t molla_sample_policy_loss(const void *d_logits, int32_t logits_type, int6
 
 int64_t molla_sample_preference_workspace_bytes(int32_t B) {
     if (B < 0) return fail(MOLLA_ERR_ARGUMENT, "bad shape for the workspace query%s");
-    return (((int64_t)B * 12 + 255) / 256 + 1) * 256;   // the rows' stats and derivatives
+    return (((int64_t)B * 16 + 255) / 256 + 1) * 256;   // the rows' stats, derivatives and what rounding their logprobs leaves out
 }
 
 int32_t molla_sample_preference_loss(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V,
@@ -2647,13 +2647,13 @@ int32_t molla_sample_preference_loss(const void *d_logits, int32_t logits_type, 
         return fail(MOLLA_ERR_WORKSPACE, "workspace missing or too small%s");
     if ((uintptr_t)d_workspace % 8) return fail(MOLLA_ERR_ARGUMENT, "the workspace has to start on a multiple of 8 bytes%s");
     if (d_grad_logits && (rc = loss_gradient(a, d_grad_logits, grad_stride)) != MOLLA_OK) return rc;
-    float *stats = (float *)d_workspace, *g = stats + 2 * (int64_t)B;
+    float *stats = (float *)d_workspace, *g = stats + 2 * (int64_t)B, *lo = g + (int64_t)B;
     LossArgs score = a;
     score.grad = nullptr;
-    score.logprob = d_logprob; score.status = d_row_status; score.stats = stats;
+    score.logprob = d_logprob; score.logprob_lo = lo; score.status = d_row_status; score.stats = stats;
     cudaError_t e = molla_loss_score(score, (cudaStream_t)stream);
     PairArgs p = {};
-    p.B = B; p.n_pairs = n_pairs; p.tokens = d_tokens; p.off = d_seq_off; p.logprob = d_logprob; p.ref_logprob = d_ref_logprob;
+    p.B = B; p.n_pairs = n_pairs; p.tokens = d_tokens; p.off = d_seq_off; p.logprob = d_logprob; p.logprob_lo = lo; p.ref_logprob = d_ref_logprob;
     p.weight = d_pair_weight; p.row_status = d_row_status;
     p.beta = beta; p.smoothing = label_smoothing; p.scale = scale; p.grad_scale = grad_scale;
     p.loss = d_loss; p.pair_loss = d_pair_loss; p.margin = d_margin; p.seq_logratio = d_seq_logratio; p.pair_status = d_pair_status;

@@ -582,6 +582,25 @@ def test_the_widest_rows(dev, lib, dtype):
         losses.token_logprobs(torch.zeros((1, V + 1), dtype=dtype, device=dev), tok[:1])
 
 
+@pytest.mark.parametrize("B", [1, 2, 9, 24, 70, 150])
+def test_the_widest_rows_for_any_number_of_rows(dev, lib, B):
+    """Every layout that the number of rows chooses, at the width where least shared memory is left."""
+    V = 720896
+    x, tok, gen = make(1, V, torch.float32, dev, seed=37)
+    x, tok = x.expand(B, V).contiguous(), tok.expand(B).contiguous()
+    ref = Rows(x[:1], tok[:1])
+    got = losses.token_logprobs(x, tok, want_entropy=True)
+    close(got["logprob"], ref.l.expand(B), ref.err_l.expand(B))
+    close(got["entropy"], ref.H.expand(B), ref.err_H.expand(B))
+    adv = torch.ones(B, device=dev)
+    want, off = ref.gradient(-adv[:1], err_g=2 * ref.err_l)
+    back = losses.token_logprobs_backward(x, tok, got, -adv)
+    p = losses.policy_loss(x, tok, got["logprob"], adv, out=x)
+    for r in range(B):
+        close(back[r:r + 1], want, off)
+        close(p["grad_logits"][r:r + 1], want, off)
+
+
 def test_rows_further_apart_than_32_bits_count(dev, lib):
     """A row that begins 2^31 + 2^20 elements into its block, for the logits and for the gradient."""
     V, step = 40000, 2**30 + 2**19
