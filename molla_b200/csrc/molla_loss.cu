@@ -339,14 +339,14 @@ constexpr float LATE = -1.0f;
 // The sum over a warp of values from 0 to 64, to 2^-38 each: in integers of 2^-16 and, for what that leaves, of 2^-38 (the bits that an addition
 // to 192, or to 1.5 2^-15, ends in), which add up exactly in whatever order. (A tree of 32-bit sums loses what is below half a step of the
 // largest value, always downwards: 5e-8 of a unit, which the log ratio of a long sequence adds up.) A NaN stays.
-__device__ __forceinline__ Two warp_sum_exact(float v) {
-    const float high = __fadd_rn(v, 192.0f), left = __fsub_rn(v, __fsub_rn(high, 192.0f)), low = __fadd_rn(left, 1.5f / 32768.0f);
+__device__ __forceinline__ Two warp_sum_exact(Two t) {
+    const float v = t.hi, high = __fadd_rn(v, 192.0f), left = __fadd_rn(__fsub_rn(v, __fsub_rn(high, 192.0f)), t.lo), low = __fadd_rn(left, 1.5f / 32768.0f);
     const int A = __reduce_add_sync(0xffffffffu, __float_as_int(high) - __float_as_int(192.0f));
     const int B = __reduce_add_sync(0xffffffffu, __float_as_int(low) - __float_as_int(1.5f / 32768.0f));
     const Two s = two_sum((float)(A >> 8) * (1.0f / 256.0f), __fmaf_rn((float)B, 1.0f / 274877906944.0f, (float)(A & 255) * (1.0f / 65536.0f)));
     return __any_sync(0xffffffffu, !(v <= 64.0f)) ? Two{NAN, 0.0f} : s;
 }
-__device__ __forceinline__ void put_sum(Stat &o, float v) {
+__device__ __forceinline__ void put_sum(Stat &o, Two v) {
     const Two s = warp_sum_exact(v);
     o.s = s.hi;
     o.s_lo = o.m == -INFINITY ? s.lo : __fmaf_rn(EX2_LOW, s.hi - 1.0f, s.lo);
@@ -367,20 +367,31 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
     Stat o;
     o.m = warp_max(Chunk<T>::top(Chunk<T>::max(Chunk<T>::max(most.x, most.y), Chunk<T>::max(most.z, most.w))));
     const float m = o.m == -INFINITY ? 0.0f : o.m;   // nothing but -inf (and NaN): sums of 0 (and NaN)
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll(FULL ? KU / 2 : 1)
-    for (int k = 0; k < KU; k++)
-        if (FULL || k * 32 + lane < chunks) {
-            float x[Chunk<T>::N];
-            Chunk<T>::get(lds16(slot + k * 512 + lane * 16), x);
+    // Sixteen logits at a time are added up in 32 bits, their sums with what that rounds off: where one logit has most of the sum, every addition to
+    // it would lose up to half a step, and what is smaller than that altogether (the logprobs of 128256 bf16 logits were low by 1.5e-8 on the
+    // average, with a standard error of 3.8e-8; so they are right to 1e-9 on the average, with 2.7e-8, for 1 % of the time).
+    constexpr int CHUNKS = 16 / Chunk<T>::N;
+    Two sum{0.0f, 0.0f};
+    float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll(FULL ? KU / 2 / CHUNKS : 1)
+    for (int k0 = 0; k0 < KU; k0 += CHUNKS) {
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < Chunk<T>::N; i++) {
-                const float d = __fsub_rn(x[i], m), e = ex2(d * c);
-                s[i & 3] += e;
-                if (ENT) w[i & 3] = __fmaf_rn(e, d < DEEP ? DEEP : d, w[i & 3]);
+        for (int k = k0; k < k0 + CHUNKS; k++)
+            if (FULL || k * 32 + lane < chunks) {
+                float x[Chunk<T>::N];
+                Chunk<T>::get(lds16(slot + k * 512 + lane * 16), x);
+#pragma unroll
+                for (int i = 0; i < Chunk<T>::N; i++) {
+                    const float d = __fsub_rn(x[i], m), e = ex2(d * c);
+                    s[i & 3] = k == k0 && i < 4 ? e : s[i & 3] + e;
+                    if (ENT) w[i & 3] = __fmaf_rn(e, d < DEEP ? DEEP : d, w[i & 3]);
+                }
             }
-        }
-    put_sum(o, (s[0] + s[1]) + (s[2] + s[3]));
+        const Two next = two_sum(sum.hi, (s[0] + s[1]) + (s[2] + s[3]));
+        sum = Two{next.hi, sum.lo + next.lo};
+    }
+    put_sum(o, sum);
     o.w = 0.0f;
     if (ENT) {
         const float ws = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
@@ -394,7 +405,7 @@ template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) 
     Stat o;
     o.m = warp_max(x);
     const float m = o.m == -INFINITY ? 0.0f : o.m, d = __fsub_rn(x, m), e = ex2(d * c);
-    put_sum(o, e);
+    put_sum(o, Two{e, 0.0f});
     o.w = ENT ? warp_sum(e * (d < DEEP ? DEEP : d)) : 0.0f;
     return o;
 }
