@@ -406,7 +406,8 @@ int32_t molla_sample_sharded_step(void *comm, int32_t rank, int32_t world, const
  * makes everything of its row NaN, the gradient too.
  *
  * d_grad_logits (NULL = not wanted) takes the gradient in the logits' type, rows grad_stride elements apart. It
- * may be the logits themselves (same address, same stride), which are then overwritten; any other overlap is refused.
+ * may be the logits themselves (same address, same stride), which are then overwritten; any other overlap is refused. No other
+ * output may lie in the place of an input.
  * Gradient rows whose factor is zero are zeros without the logits being read, whatever they hold.
  *
  * Everything within a row is held in 32 bits or more, sums over rows in 64 bits, each in an order of its own that

@@ -108,20 +108,25 @@ __device__ __forceinline__ Two ln_of(float S) {
     return two_sum(n * LN2_SHORT, __fmaf_rn(n, LN2_REST, y));
 }
 
-// exp(q) - 1 - q: for small q from its series, which the difference would lose
-__device__ __forceinline__ float exp_less_line(float q) {
-    if (fabsf(q) > 0.5f) return __fsub_rn(expm1f(q), q);
+// exp(q) - 1 - q, for small q from its series, which the difference would lose, and exp(q) - 1
+__device__ __forceinline__ float exp_less_line(float q, float &less_one) {
+    if (fabsf(q) > 0.5f) {
+        less_one = expm1f(q);
+        return isinf(less_one) ? less_one : __fsub_rn(less_one, q);
+    }
     float p = 1.0f / 3628800.0f;
     p = __fmaf_rn(p, q, 1.0f / 362880.0f); p = __fmaf_rn(p, q, 1.0f / 40320.0f); p = __fmaf_rn(p, q, 1.0f / 5040.0f);
     p = __fmaf_rn(p, q, 1.0f / 720.0f); p = __fmaf_rn(p, q, 1.0f / 120.0f); p = __fmaf_rn(p, q, 1.0f / 24.0f);
     p = __fmaf_rn(p, q, 1.0f / 6.0f); p = __fmaf_rn(p, q, 0.5f);
-    return p * q * q;
+    p = p * q * q;
+    less_one = p + q;
+    return p;
 }
 
 // What a row answers once its maximum M, sum S and, where entropies are wanted, W are known: first what its gradient
 // waits for, all of it in 32 bits (conversions to 64 run where the exponentials do, behind theirs: with 64 bits, logarithm, exponential and
 // divisions a row's blocks waited 6200 cycles, with conversions alone 2400), then the rest.
-struct Answer { unsigned int status; Two l, lnS; float mean, ratio, q, kl; bool held; };
+struct Answer { unsigned int status; Two l, lnS; float mean, ratio, kl; bool held; };
 
 template <bool ENT>
 __device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in, float M, Two S, float W, float depth, float c, Answer &o) {
@@ -136,24 +141,25 @@ __device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in
     o.lnS.lo = __fmaf_rn(off, depth, o.lnS.lo);
     const float nats = in.per_T, nats_lo = __fmaf_rn(-in.T, nats, 1.0f) * nats, dx = __fsub_rn(in.xt, M);
     o.mean = ENT ? W * per_S * nats : 0.0f;
-    if (ordinary(dx) && ordinary(o.lnS.hi)) {
+    const float p = dx * nats;
+    if (ordinary(p) && ordinary(o.lnS.hi)) {
         const Two d = two_sum(in.xt, -M);
-        const float p = dx * nats, p_lo = __fmaf_rn(dx, nats, -p) + __fmaf_rn(dx, nats_lo, d.lo * nats);
+        const float p_lo = __fmaf_rn(dx, nats, -p) + __fmaf_rn(dx, nats_lo, d.lo * nats);
         const Two s = two_sum(p, -o.lnS.hi);
         o.l = two_sum(s.hi, s.lo + (p_lo - o.lnS.lo));
     } else {
-        o.l = Two{dx * nats - o.lnS.hi, 0.0f};
+        o.l = Two{p - o.lnS.hi, 0.0f};
     }
-    o.ratio = o.q = o.kl = 0.0f;
+    o.ratio = o.kl = 0.0f;
     o.held = false;
     if (!a.row_loss) return RowGrad{0.0f, 0.0f, 0.0f};
     o.ratio = expf((o.l.hi - in.old) + o.l.lo);
     o.held = (in.advantage > 0.0f && o.ratio > 1.0f + a.clip_high) || (in.advantage < 0.0f && o.ratio < 1.0f - a.clip_low);   // (not a NaN)
     float g = o.held ? 0.0f : -(o.ratio * in.advantage);
     if (a.ref_logprob) {
-        o.q = (in.ref - o.l.hi) - o.l.lo;
-        o.kl = exp_less_line(o.q);
-        if (a.kl_coef != 0.0f) g = __fmaf_rn(-a.kl_coef, o.kl + o.q, g);
+        float less_one;
+        o.kl = exp_less_line((in.ref - o.l.hi) - o.l.lo, less_one);
+        if (a.kl_coef != 0.0f) g = __fmaf_rn(-a.kl_coef, less_one, g);
     }
     const float by = in.weight * a.scale * a.grad_scale;
     return o.status ? RowGrad{0.0f, 0.0f, 0.0f} : row_grad(g * by, ENT ? -a.entropy_coef * by : 0.0f, in.per_T, per_S, o.mean);

@@ -229,6 +229,37 @@ def test_policy_loss(dev, lib, B, V, dtype, terms):
         assert torch.equal(none[n], got[n]) and torch.equal(place[n], got[n]), n
 
 
+def test_old_and_reference_logprobs_far_from_the_rows_own(dev, lib):
+    """Impossible tokens and infinite logprobs: what the formulas give, row by row."""
+    V = 300
+    x, tok, gen = make(7, V, torch.float32, dev, seed=41)
+    x[5] = 0.0
+    x[5, int(tok[5])] = -math.inf                      # a token that cannot be: ratio 0, KL infinite
+    x[6] = 0.0
+    x[6, int(tok[6])], x[6, int(tok[6]) - 1] = -3e38, 3e38   # one whose logprob is beyond 32 bits
+    l = losses.token_logprobs(x, tok)["logprob"]
+    assert l[5] == -math.inf and l[6] == -math.inf and bool(l[:5].isfinite().all())
+    inf = math.inf
+    old = torch.tensor([-inf, -inf, 0.0, 0.0, 0.0, 0.0, 0.0], device=dev)
+    old[2:5] = l[2:5]
+    ref = l.clone()
+    ref[2], ref[3] = -inf, l[3] + 200.0
+    ref[5:] = 0.0
+    adv = torch.tensor([1.0, -1.0, 1.0, 1.0, 0.0, -1.0, 1.0], device=dev)
+    got = losses.policy_loss(x, tok, old, adv, ref_logprob=ref, kl_coef=0.5)
+    assert got["clipped"].tolist() == [True, False, False, False, False, True, False]
+    row, kl, grad = got["row_loss"].tolist(), got["kl"].tolist(), got["grad_logits"]
+    # the clip holds an infinite ratio; what is left is the KL term's, whose q is the rounding of the reference logprob, half a step of it
+    assert abs(row[0] + 1.2) < 2e-7 and bool((grad[0].abs() <= 0.5 * 1.01 * float(l[0].abs()) * U).all())
+    assert row[1] == inf and not grad[1].isfinite().all()
+    assert kl[2] == inf and row[2] == inf                         # exp(q) - 1 is -1: the gradient is finite
+    R = Rows(x[2:3], tok[2:3])
+    close(grad[2:3], *R.gradient(torch.tensor([-1.0 + 0.5], device=dev), err_g=2 * R.err_l))
+    assert kl[3] == inf and row[3] == inf
+    assert abs(row[4]) < 1e-6 and not bool((grad[4].abs() > 1e-6).any())
+    assert kl[5] == inf and kl[6] == inf
+
+
 def test_the_clip_on_either_side(dev, lib):
     """Ratios of 1/2, 1 and 2 for advantages of either sign, one of zero, and clip ranges that are not alike."""
     V = 500
