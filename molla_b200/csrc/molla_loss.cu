@@ -1067,14 +1067,15 @@ Layout layout_with(int C, int W, int per_sm, int V, int size) {
 // 123 / 111, 8288 x 128256 bf16 395 / 381, 4096 x 128256 fp32 350 / 339.
 //
 // Where a row's units come a second time, out of L2, as many blocks share a row as keep what is in flight below 96 MB: 1 / 2 / 4 blocks a row took
-// 529 / 560 / 675 us for 4096 x 151936 bf16 (304 KB a row), 488 / 405 / 419 for 2072 x 128256 fp32 (513 KB), 519 / 495 / 413 for 1024 x 262144 fp32
-// (1 MB). Few rows are shared by as many blocks as there is room for: 4 x 32000 fp32 19.5 / 17.4 / 15.4, by eight 15.4.
-constexpr long long IN_FLIGHT = 96ll << 20;
+// 532 / 575 / 675 us for 4096 x 151936 bf16 (304 KB a row), 507 / 468 / - for 2048 x 262144 bf16 (524 KB), 480 / 402 / 418 for 2072 x 128256 fp32
+// (513 KB), 519 / 495 / 413 for 1024 x 262144 fp32 (1 MB). Of fp32 rows, which have less to compute and so feel what L2 loses more, two share a row from 60 MB on:
+// 329 / 288 for 3000 x 65536 (77 MB), 200 / 223 for 4096 x 32000 (38 MB). Few rows are shared by as many blocks as there is room for: 4 x 32000 fp32
+// 19.5 / 17.4 / 15.4, by eight 15.4.
 template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms) {
     const int size = (int)sizeof(T), most = (int)(((long long)V * size + UB - 1) / UB);
     int C = 1;
     if (STATS && GRAD)
-        while (C < 8 && (most + C - 1) / C > 18 && 2ll * sms / C * most * UB > IN_FLIGHT) C *= 2;
+        while (C < 8 && (most + C - 1) / C > 18 && 2ll * sms / C * most * UB > (size == 4 && C == 1 ? 60ll : 96ll) << 20) C *= 2;
     while (C < 8 && 2ll * B * C <= 2ll * sms * 15 / 16 && most >= 8 * C) C *= 2;
     const int share = (most + C - 1) / C;
     int W = share <= 4 ? share : share <= 18 ? (share + 1) / 2 : STATS ? 13 : 16;
