@@ -393,7 +393,7 @@ int32_t molla_sample_sharded_step(void *comm, int32_t rank, int32_t world, const
  * the reference, which serves and does not train; they start where it stops: the tokens that
  * `Sampler.pick` chose and the logprobs `Sampler.logprobs` gives them (src/molla/engine/sample.mojo:268-359).
  *
- * All of them read a block of B rows of V logits of type `logits_type` (MOLLA_LOGITS_*), row r at
+ * All of them read a block of B rows (at most 2^30) of V logits of type `logits_type` (MOLLA_LOGITS_*), row r at
  * d_logits + r*row_stride elements, at most 720896 logits a row, and one token a row, d_tokens [B] int32, as
  * molla_sample_batch leaves them. With z = logits / temperature of the row (d_temperature [B], NULL = 1;
  * it has to be finite and above zero) the distribution of a row is softmax(z),

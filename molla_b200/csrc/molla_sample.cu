@@ -1817,6 +1817,7 @@ int loss_block(LossArgs &a, const void *logits, int type, int64_t row_stride, in
     if (!logits || !tokens) return fail(MOLLA_ERR_ARGUMENT, "logits and tokens are required%s");
     if (type != MOLLA_LOGITS_FP32 && type != MOLLA_LOGITS_BF16 && type != MOLLA_LOGITS_FP16) return fail(MOLLA_ERR_ARGUMENT, "logits are fp32, bf16 or fp16%s");
     if (B < 0 || V <= 0 || row_stride < V) return fail(MOLLA_ERR_ARGUMENT, "bad block shape%s");
+    if (B > 1 << 30) return fail(MOLLA_ERR_ARGUMENT, "more than 2^30 rows%s");   // (the stats' places are counted in 32 bits)
     if (V > MAX_VOCAB) return fail(MOLLA_ERR_VOCAB, "vocabulary too wide%s");
     if ((uintptr_t)logits % (type == MOLLA_LOGITS_FP32 ? 4 : 2)) return fail(MOLLA_ERR_ARGUMENT, "logits have to be aligned to their type%s");
     a.logits = logits; a.type = type; a.row_stride = row_stride; a.B = B; a.V = V;

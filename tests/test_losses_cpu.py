@@ -39,7 +39,7 @@ def preference(L, off=P, pairs=1, beta=0.1, smoothing=0.0, scale=1.0, grad_scale
 @pytest.mark.parametrize("call", [score, backward, policy, preference])
 @pytest.mark.parametrize("bad,code", [
     (dict(logits=NULL), capi.ERR_ARGUMENT), (dict(tokens=NULL), capi.ERR_ARGUMENT), (dict(kind=3), capi.ERR_ARGUMENT),
-    (dict(kind=-1), capi.ERR_ARGUMENT), (dict(B=-1), capi.ERR_ARGUMENT), (dict(V=0), capi.ERR_ARGUMENT),
+    (dict(kind=-1), capi.ERR_ARGUMENT), (dict(B=-1), capi.ERR_ARGUMENT), (dict(B=2**30 + 1), capi.ERR_ARGUMENT), (dict(V=0), capi.ERR_ARGUMENT),
     (dict(stride=7), capi.ERR_ARGUMENT), (dict(V=720897, stride=720897), capi.ERR_VOCAB),
     (dict(logits=C.c_void_p(4098)), capi.ERR_ARGUMENT), (dict(kind=1, logits=C.c_void_p(4097)), capi.ERR_ARGUMENT)])
 def test_blocks_against_the_rules(lib, call, bad, code):
