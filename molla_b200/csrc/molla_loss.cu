@@ -1071,6 +1071,13 @@ Layout layout_with(int C, int W, int per_sm, int V, int size) {
 // (513 KB), 519 / 495 / 413 for 1024 x 262144 fp32 (1 MB). Of fp32 rows, which have less to compute and so feel what L2 loses more, two share a row from 60 MB on:
 // 329 / 288 for 3000 x 65536 (77 MB), 200 / 223 for 4096 x 32000 (38 MB). Few rows are shared by as many blocks as there is room for: 4 x 32000 fp32
 // 19.5 / 17.4 / 15.4, by eight 15.4.
+//
+// Many rows of a block each: five or nine warps with the one that answers leave one of an SM's four schedulers most of the work, and where the rounds of
+// 13 do not come out even, seven in four blocks idle less. Usual / as here, us, 400 MB of logits: score, bf16, units a row 10, 15, 19, 25: 115 / 97, 107 / 94,
+// 98 / 94, 101 / 96 (13: 98 / 96, and 40 / 45 with only 2450 rows: seven stay); backward 4, 10, 18: 162 / 151, 156 / 149, 150 / 145; policy loss with
+// its gradient, bf16, four in six blocks though the units do not stay, 15, 18, 20, 24: 228 / 196, 208 / 191, 218 / 187, 189 / 181 (16, eight in three: 198 / 202;
+// fp32, 15, 18: 158 / 168, 145 / 176); seven in four for 28, 40: 224 / 189, 202 / 187, fp32 173 / 159, 160 / 178; eleven in two, whose rounds are
+// three warps a scheduler, not four, for 63, 75 of bf16: 185 / 179, 530 / 516 (4096 rows), for 50, 16 against 15 of them: 188 / 203.
 template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms) {
     const int size = (int)sizeof(T), most = (int)(((long long)V * size + UB - 1) / UB);
     int C = 1;
@@ -1081,7 +1088,27 @@ template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms
     int W = share <= 4 ? share : share <= 18 ? (share + 1) / 2 : STATS ? 13 : 16;
     if (STATS && !GRAD && (long long)B * C > sms) W = even(share, share <= 6 ? (share + 1) / 2 : 7);
     else if (W < 13) W = even(share, W);
-    const int per_sm = W >= 13 ? 2 : 32 / (W + 1);
+    int per_sm = W >= 13 ? 2 : 32 / (W + 1);
+    const auto rounds = [&](int w) { return (share + w - 1) / w; };
+    const long long rows_per_sm = C == 1 ? B / sms : 0;
+    if (!STATS && W != 7 && share >= 4 && share <= 18 && rows_per_sm >= 16) {
+        W = 4;
+        per_sm = 8;
+    } else if (STATS && !GRAD && size == 2 && W != 7 && share > 7 && share <= 32 && rows_per_sm >= 16) {
+        W = 3;
+        per_sm = 8;
+    } else if (STATS && GRAD && size == 2 && W != 7 && W != 8 && share >= 13 && share <= 24 && rows_per_sm >= 12) {
+        W = 4;
+        per_sm = 6;
+    } else if (STATS && GRAD && share > 18 && rows_per_sm >= 8) {
+        const int usual = even(share, W);
+        if (share <= (size == 4 ? 28 : 41) && even(share, 7) == 7 && 40 * rounds(usual) > 23 * rounds(7)) {
+            W = 7;
+            per_sm = 4;
+        } else if (size == 2 && share > 41 && even(share, 11) == 11 && 10 * 3 * rounds(11) <= 9 * ((usual + 3) / 4) * rounds(usual)) {
+            W = 11;
+        }
+    }
     return layout_with(C, W, per_sm < 10 ? per_sm : 10, V, size);
 }
 

@@ -297,6 +297,30 @@ def test_a_rollout_scored_by_the_policy_that_made_it_has_ratios_of_one(dev, lib)
             assert bool(((got["row_loss"] + adv).abs() <= adv.abs() * (all_rows["logprob"].abs() * U + 2 * U)).all())
 
 
+@pytest.mark.parametrize("B,V,dtype", [(2400, 30001, torch.bfloat16), (2400, 9001, torch.float32), (1200, 28601, torch.float32),
+                                       (1200, 57201, torch.float16), (1200, 129000, torch.bfloat16)])
+def test_rows_among_many_are_what_they_are_among_few(dev, lib, B, V, dtype):
+    """The same bits, whatever the number of rows makes of their way through the device; in place as well."""
+    x, tok, gen = make(B, V, dtype, dev, seed=B + V)
+    old, ref, adv, g, h = (normal(gen, B, dev) for _ in range(5))
+    T = 0.5 + torch.rand(B, generator=gen, device=dev)
+    tok[7::13] = -1
+
+    def calls(s):
+        scored = losses.token_logprobs(x[s], tok[s], T[s], want_entropy=True)
+        grad = losses.token_logprobs_backward(x[s], tok[s], scored, g[s], h[s], T[s])
+        plain = losses.token_logprobs(x[s], tok[s], T[s])["logprob"]
+        pol = losses.policy_loss(x[s], tok[s], old[s], adv[s], ref_logprob=ref[s], kl_coef=0.1, entropy_coef=0.01, temperature=T[s])
+        place = x[s].clone()
+        losses.policy_loss(place, tok[s], old[s], adv[s], out=place)
+        return [scored["logprob"], scored["entropy"], grad, plain, pol["row_loss"], pol["logprob"], pol["entropy"], pol["grad_logits"], place]
+
+    many = calls(slice(0, B))
+    for s in (slice(0, 24), slice(B // 2, B // 2 + 40), slice(B - 24, B)):
+        for k, (a, b) in enumerate(zip(many, calls(s))):
+            assert torch.equal(a[s].view(torch.uint8 if a.dim() > 1 else a.dtype), b.view(torch.uint8 if b.dim() > 1 else b.dtype)), (k, s)
+
+
 # ---- the preference loss ---------------------------------------------------------------------------------
 
 def preference_reference(x, tok, off, ref=None, w=None, beta=0.1, eps=0.0, T=None, scale=1.0, grad_scale=1.0):
