@@ -7,9 +7,9 @@ They start where the sampling calls stop. A rollout's tokens and old logprobs:
     old = losses.token_logprobs(logits, out["tokens"], temperature=params["temperature"])["logprob"]
 
 (`chosen_logprob` is of the logits as the model gave them; rows drawn at a temperature have the logprobs of that
-temperature.) A training step, for logits that an autograd graph made:
+temperature; greedy rows, of temperature 0, have none and are scored at one above it.) A training step, for logits that an autograd graph made:
 
-    got = losses.policy_loss(logits.detach(), tokens, old, advantage, weight=mask, scale=1 / n_tokens)
+    got = losses.policy_loss(logits.detach(), tokens, old, advantage, weight=mask, temperature=temperature, scale=1 / n_tokens)
     logits.backward(got["grad_logits"])
 
 Loss and gradient come from one call; nothing here takes part in autograd. Calls are asynchronous on the
