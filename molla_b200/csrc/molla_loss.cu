@@ -358,13 +358,14 @@ __device__ __forceinline__ void put_sum(Stat &o, Two v) {
     o.s_lo = o.m == -INFINITY ? s.lo : __fmaf_rn(EX2_LOW, s.hi - 1.0f, s.lo);
 }
 
-// A unit's, from shared memory twice: once for its maximum, then for the sums (four of either a lane).
-template <class T, bool ENT, bool FULL>
+// A unit's, from shared memory twice: once for its maximum, then for the sums (four of either a lane). PART: how many sums of a unit that is not full
+// are unrolled: as many as of a full one (8288 x 128256 bf16 392 to 383 us) but with a gradient, whose registers would spill (1 % slower).
+template <class T, bool ENT, bool FULL, int PART>
 __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
     const int lane = threadIdx.x & 31;
     constexpr unsigned int low = Chunk<T>::LOWEST;
     uint4 most = make_uint4(low, low, low, low);
-#pragma unroll(FULL ? KU / 2 : 1)
+#pragma unroll(FULL ? KU / 2 : PART)
     for (int k = 0; k < KU; k++)
         if (FULL || k * 32 + lane < chunks) {
             const uint4 v = lds16(slot + k * 512 + lane * 16);
@@ -379,7 +380,7 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
     constexpr int CHUNKS = 16 / Chunk<T>::N;
     Two sum{0.0f, 0.0f};
     float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll(FULL ? KU / 2 / CHUNKS : 1)
+#pragma unroll(FULL ? KU / 2 / CHUNKS : PART)
     for (int k0 = 0; k0 < KU; k0 += CHUNKS) {
         float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -853,7 +854,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
             const bool tell = lane < (GRAD ? L.C : 1);   // a lane a block that wants to know
             for (int u = warp; u < span.units; u += warps) {
                 const uint32_t slot = feed.wait(held + units);
-                Stat o = u < span.full ? unit_stat<T, ENT, true>(slot, 0, c) : unit_stat<T, ENT, false>(slot, span.last_chunks(), c);
+                Stat o = u < span.full ? unit_stat<T, ENT, true, 1>(slot, 0, c) : unit_stat<T, ENT, false, GRAD ? 1 : 2>(slot, span.last_chunks(), c);
                 if (feed.late || LOSS_KNOB(a, 16)) o.s_lo = LATE;   // (testing build: a wait that ran out)
                 if (tell) put16(alone, st + u, lane, o.m, o.s, o.w, o.s_lo, &ctl.sums[s]);
                 if (GRAD && L.resident) units++;
