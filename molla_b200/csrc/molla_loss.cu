@@ -1,10 +1,11 @@
 // Logprobs of given tokens, their gradient, and the losses over them (the formulas: include/molla_sample.h).
 //
-// With M = max x, c = log2(e)/T and e_j = 2^(c (x_j - M)), S = sum e_j and W = sum e_j (x_j - M):
-//     logprob = (x_t - M)/T - ln S        entropy = ln S - W/(S T)        p_j = e_j/S
+// With M = max x, c = log2(e)/T, t_j = c (x_j - M) and e_j = 2^t_j, S = sum e_j and W = sum e_j t_j:
+//     logprob = (x_t - M)/T - ln S        entropy = ln S - W/(S c T)        p_j = e_j/S
 // and for g = dL/dlogprob, h = dL/dentropy the gradient by logit j is
-//     g [j = t]/T - e_j (A + H (x_j - M))   with  H = h/(T T S),  A = (g - h W/(S T))/(T S)
-// so a row needs three numbers (M, S, W) for everything. Differences from M are exact for the logits that matter, and
+//     g [j = t]/T - e_j (A + H t_j)   with  H = h/(c T T S),  A = (g - h W/(S c T))/(T S)
+// so a row needs three numbers (M, S, W) for everything. What multiplies e_j is counted in its exponent, not in x_j - M: t_j can be held at a
+// number as small as -160, where e_j is 0 whatever the temperature, so that no product of a masked logit leaves 32 bits. Differences from M are exact for the logits that matter, and
 // whatever rounding e_j has is the same in S and in the gradient, where it cancels to first order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -28,7 +29,7 @@ namespace {
 
 constexpr double LOG2E_64 = 1.44269504088896340736;
 constexpr float LOG2E = (float)LOG2E_64, LOG2E_LEFT = (float)(LOG2E_64 - (double)LOG2E);
-constexpr float DEEP = -1e30f;    // where x - M is held, so that 0 * (x - M) is 0 for logits of -inf too
+constexpr float DEEP = -160.0f;   // where an exponent is held as a factor: 2^t is 0 below -126 (-150 with subnormals), and 0 * t stays 0 for logits of -inf
 constexpr unsigned int ROW_ERRORS = MOLLA_ROW_BAD_TOKEN | MOLLA_ROW_EMPTY | MOLLA_ROW_INVALID_CONFIG | MOLLA_ROW_LOAD_TIMEOUT;
 
 // Kernels of one call begin when the one before is about to end, and wait here until it has.
@@ -76,15 +77,23 @@ __device__ __forceinline__ RowIn row_in(const LossArgs &a, int r) {
     return in;
 }
 
-// The gradient's three numbers: add at the token, and A and H of the formula; `mean` is W/(S T).
+// 1/(c T): ln 2, but for what rounding left out of c.
+__device__ __forceinline__ float nats_of(float c, float T) { return __frcp_rn(__fmul_rn(c, T)); }
+
+// The gradient's three numbers: add at the token, and A and H of the formula; `mean` is W/(S c T). Finite derivatives over a temperature near
+// the least one would leave 32 bits: the three are held at what a probability of 0 still makes 0 of (|H| 160 + |A| is below the largest float).
 struct RowGrad { float token, A, H; };
 
-__device__ __forceinline__ RowGrad row_grad(float g, float h, float per_T, float per_S, float mean) {
+__device__ __forceinline__ bool ordinary(float x) { return fabsf(x) < 3e38f; }
+__device__ __forceinline__ float held_at(float x, float most) { return fabsf(x) > most ? copysignf(most, x) : x; }   // (NaN stays)
+
+__device__ __forceinline__ RowGrad row_grad(float g, float h, float per_T, float per_S, float mean, float nats) {
     RowGrad o;
     const float inv = per_T * per_S;
     o.token = g * per_T;
     o.A = __fmaf_rn(-h, mean, g) * inv;
-    o.H = h * inv * per_T;
+    o.H = h * inv * nats;
+    if (ordinary(g) && ordinary(h)) { o.token = held_at(o.token, 1.6e38f); o.A = held_at(o.A, 1.6e38f); o.H = held_at(o.H, 1e36f); }
     return o;
 }
 
@@ -94,7 +103,6 @@ __device__ __forceinline__ Two two_sum(float a, float b) {
     const float s = __fadd_rn(a, b), bb = __fsub_rn(s, a);
     return Two{s, __fadd_rn(__fsub_rn(a, __fsub_rn(s, bb)), __fsub_rn(b, bb))};
 }
-__device__ __forceinline__ bool ordinary(float x) { return fabsf(x) < 3e38f; }
 
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float LN2_SHORT = 0.693145751953125f, LN2_REST = (float)(0.693147180559945309 - 0.693145751953125);   // 17 bits, times a small integer exact
@@ -140,7 +148,8 @@ __device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in
     const float off = (__fmaf_rn(c, in.T, -LOG2E) - LOG2E_LEFT) * LN2;
     o.lnS.lo = __fmaf_rn(off, depth, o.lnS.lo);
     const float nats = in.per_T, nats_lo = __fmaf_rn(-in.T, nats, 1.0f) * nats, dx = __fsub_rn(in.xt, M);
-    o.mean = ENT ? W * per_S * nats : 0.0f;
+    const float per_cT = ENT ? nats_of(c, in.T) : 0.0f;
+    o.mean = ENT ? W * per_S * per_cT : 0.0f;
     const float p = dx * nats;
     if (ordinary(p) && ordinary(o.lnS.hi)) {
         const Two d = two_sum(in.xt, -M);
@@ -162,7 +171,7 @@ __device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in
         if (a.kl_coef != 0.0f) g = __fmaf_rn(-a.kl_coef, less_one, g);
     }
     const float by = in.weight * a.scale * a.grad_scale;
-    return o.status ? RowGrad{0.0f, 0.0f, 0.0f} : row_grad(g * by, ENT ? -a.entropy_coef * by : 0.0f, in.per_T, per_S, o.mean);
+    return o.status ? RowGrad{0.0f, 0.0f, 0.0f} : row_grad(g * by, ENT ? -a.entropy_coef * by : 0.0f, in.per_T, per_S, o.mean, per_cT);
 }
 
 __device__ __forceinline__ void row_write(const LossArgs &a, int r, const RowIn &in, float M, float S, const Answer &o) {
@@ -390,9 +399,9 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
                 Chunk<T>::get(lds16(slot + k * 512 + lane * 16), x);
 #pragma unroll
                 for (int i = 0; i < Chunk<T>::N; i++) {
-                    const float d = __fsub_rn(x[i], m), e = ex2(d * c);
+                    const float t = __fsub_rn(x[i], m) * c, e = ex2(t);
                     s[i & 3] = k == k0 && i < 4 ? e : s[i & 3] + e;
-                    if (ENT) w[i & 3] = __fmaf_rn(e, d < DEEP ? DEEP : d, w[i & 3]);
+                    if (ENT) w[i & 3] = __fmaf_rn(e, fmaxf(t, DEEP), w[i & 3]);
                 }
             }
         const Two next = two_sum(sum.hi, (s[0] + s[1]) + (s[2] + s[3]));
@@ -411,9 +420,9 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
 template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) {
     Stat o;
     o.m = warp_max(x);
-    const float m = o.m == -INFINITY ? 0.0f : o.m, d = __fsub_rn(x, m), e = ex2(d * c);
+    const float m = o.m == -INFINITY ? 0.0f : o.m, t = __fsub_rn(x, m) * c, e = ex2(t);
     put_sum(o, Two{e, 0.0f});
-    o.w = ENT ? warp_sum(e * (d < DEEP ? DEEP : d)) : 0.0f;
+    o.w = ENT ? warp_sum(e * fmaxf(t, DEEP)) : 0.0f;
     return o;
 }
 
@@ -439,11 +448,11 @@ template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int
     W = depth = 0.0f;
     const auto add = [&](const Stat &o) {
         const float d = o.m == -INFINITY ? 0.0f : __fsub_rn(o.m, M);   // (a unit of -inf: sums of 0, or NaN)
-        const float t = d * c, f = exp2_series(t), p = f * o.s;
+        const float t = d * c, f = exp2_series(t), p = f * o.s, held = fmaxf(t, DEEP);   // (a NaN stays in f)
         const Two s = two_sum(S.hi, p);
-        depth = __fmaf_rn(f, __fmaf_rn(t < DEEP ? -DEEP : -t, LN2 * o.s, 2.5f * fmaxf(o.s - 1.0f, 0.0f)), depth);
+        depth = __fmaf_rn(f, __fmaf_rn(-held, LN2 * o.s, 2.5f * fmaxf(o.s - 1.0f, 0.0f)), depth);
         S = Two{s.hi, S.lo + (s.lo + __fmaf_rn(f, o.s_lo, __fmaf_rn(f, o.s, -p)))};
-        if (ENT) W = __fmaf_rn(f, __fmaf_rn(d < DEEP ? DEEP : d, o.s, o.w), W);
+        if (ENT) W = __fmaf_rn(f, __fmaf_rn(held, o.s, o.w), W);
     };
 #pragma unroll
     for (int k = 0; k < HELD; k++) add(v[k]);
@@ -462,8 +471,8 @@ template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int
 
 template <class T, bool ENT>
 __device__ __forceinline__ float gradient_of(float x, float M, float c, float A, float H) {
-    const float d = __fsub_rn(x, M), e = ex2(d * c);
-    return ENT ? -(e * __fmaf_rn(H, d < DEEP ? DEEP : d, A)) : -(e * A);
+    const float t = __fsub_rn(x, M) * c, e = ex2(t);
+    return ENT ? -(e * __fmaf_rn(H, fmaxf(t, DEEP), A)) : -(e * A);
 }
 
 // One unit's gradient: `to` is where its first logit's goes.
@@ -514,7 +523,7 @@ __device__ __forceinline__ RowShare row_given(const LossArgs &a, int r) {
     o.M = a.in_stats[2 * r];
     o.c = LOG2E / T;
     const Two lnS = ln_of(S);
-    const RowGrad q = row_grad(g, h, 1.0f / T, __frcp_rn(S), h != 0.0f ? (lnS.hi - a.in_entropy[r]) + lnS.lo : 0.0f);
+    const RowGrad q = row_grad(g, h, 1.0f / T, __frcp_rn(S), h != 0.0f ? (lnS.hi - a.in_entropy[r]) + lnS.lo : 0.0f, nats_of(o.c, T));
     o.A = q.A; o.H = q.H; o.token_add = q.token;
     return o;
 }

@@ -503,6 +503,63 @@ def test_masks_inside_rows(dev, lib, V, dtype):
     assert not p["grad_logits"][gone].any() and bool(p["loss"].isfinite())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,h,grad_scale", [(1e-3, 0.01, 65536.0), (0.02, 0.01, 2.0**24), (5e-5, 1.0, 1.0), (1e-19, 1.0, 1.0), (1e-25, 0.5, 64.0),
+                                            (1e-36, 0.1, 1.0), (1.0, 0.0, 1.0), (1e36, 1.0, 1.0)])
+def test_masked_logits_at_any_temperature_and_scale(dev, lib, T, h, grad_scale, dtype):
+    """A masked logit has no gradient whatever the factor that its probability of 0 meets, and leaves the others theirs. The logits are some
+    temperatures apart, so that the rows' distributions are no matter of T."""
+    B, V = 4, 1500
+    low = torch.finfo(dtype).min
+    x, tok, gen = make(B, V, dtype, dev, seed=43)
+    if dtype is torch.float16:
+        T = min(T, 1000.0)
+    x.copy_(2.0 * T * torch.randn((B, V), generator=gen, device=dev, dtype=torch.float64))   # (what fp16 has of them: zeros, at the lowest temperatures)
+    dead = torch.rand((B, V), generator=gen, device=dev) < 0.5
+    dead[2], dead[3] = True, False
+    dead[:, 3] = False
+    tok[:] = 3
+    x[0][dead[0]] = -math.inf
+    x[1][dead[1]] = low
+    x[2][dead[2]] = -math.inf
+    temperature = torch.full((B,), T, device=dev)
+    ref = Rows(x, tok, temperature)
+    ref.rel_p = torch.where(ref.p > 0, ref.rel_p, 0.0)
+    got = losses.token_logprobs(x, tok, temperature=temperature, want_entropy=True)
+    close(got["logprob"], ref.l, ref.err_l, "logprob")
+    close(got["entropy"], ref.H, ref.err_H + 1e-300, "entropy")
+    g, hs = normal(gen, B, dev) * grad_scale, torch.full((B,), h * grad_scale, device=dev)
+    want, off = ref.gradient(g, hs)
+    off = off + ref.p * (hs.double() * (ref.err_H + ref.H.abs() * U) / ref.T)[:, None]
+    back = losses.token_logprobs_backward(x, tok, got, g, grad_entropy=hs, temperature=temperature)
+    adv = g / grad_scale
+    p = losses.policy_loss(x, tok, got["logprob"], adv, entropy_coef=h, temperature=temperature, grad_scale=grad_scale)["grad_logits"]
+    want_p, off_p = ref.gradient(-adv * grad_scale, -hs, adv.abs().double() * grad_scale * (ref.err_l + ref.err_l64) * 1.01)
+    for out, w, o in ((back, want, off), (p, want_p, off_p)):
+        assert not out[dead].any()
+        live = w.abs() < 0.9 * torch.finfo(dtype).max   # (fp16 ends at 65504)
+        close(out[live], w[live], o[live], "gradient")
+
+
+def test_masked_logits_where_the_gradient_itself_leaves_32_bits(dev, lib):
+    """50 over a temperature of 1e-38: whatever the row's own logits get, those without a probability get 0."""
+    x, tok, gen = make(3, 3000, torch.float32, dev, seed=47)
+    x *= 1e-38
+    dead = torch.rand(x.shape, generator=gen, device=dev) < 0.5
+    dead[:, 7] = False
+    dead[2] = True
+    dead[2, 7] = False
+    tok[:] = 7
+    x[dead] = -math.inf
+    T, g = torch.full((3,), 1.5e-38, device=dev), torch.full((3,), 50.0, device=dev)
+    got = losses.token_logprobs(x, tok, temperature=T, want_entropy=True)
+    for out in (losses.token_logprobs_backward(x, tok, got, g, temperature=T), losses.token_logprobs_backward(x, tok, got, g, g, temperature=T),
+                losses.policy_loss(x, tok, got["logprob"], g, temperature=T)["grad_logits"],
+                losses.policy_loss(x, tok, got["logprob"], g, entropy_coef=50.0, temperature=T)["grad_logits"]):
+        assert not out[dead].any() and not out.isnan().any()
+        assert not out[2].any()   # a row sure of its token
+
+
 def test_nan_and_infinity_stay_in_their_row(dev, lib):
     for dtype in TYPES:
         x, tok, gen = make(5, 3001, dtype, dev)
