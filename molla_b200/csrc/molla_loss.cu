@@ -1014,7 +1014,7 @@ __global__ void __launch_bounds__(ST) pairs_kernel(const __grid_constant__ PairA
         status = 0;
         for (int k = group * each; k < (group + 1) * each; k++) { sc += chosen[k]; sr += rejected[k]; status |= statuses[k]; }
         const double beta = a.beta, eps = a.smoothing, w = a.weight ? (double)a.weight[p] : 1.0, m = beta * (sc - sr);
-        const double l = w == 0.0 ? 0.0 : w * ((1.0 - eps) * soft(-m) + eps * soft(m));
+        const double l = w == 0.0 ? 0.0 : w * ((1.0 - eps) * soft(-m) + (eps == 0.0 ? 0.0 : eps * soft(m)));   // (of an infinite margin too)
         const double dm = status || w == 0.0 ? 0.0 : w * (eps * sigmoid(m) - (1.0 - eps) * sigmoid(-m));
         if (of_pair == 0) {
             total += l;

@@ -408,6 +408,31 @@ def test_margins_far_from_zero(dev, lib):
     close(got["grad_logits"][2:], *(v[2:] for v in Rows(x, tok).gradient(torch.tensor([0.0, 0.0, -1.0, 1.0], device=dev))))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_margins_of_tokens_that_cannot_be(dev, lib, dtype):
+    """A token whose logit is -inf in the rejected sequence: the margin is +inf, -ln sigmoid of it 0, and the pair adds nothing to loss
+    and gradient. In the chosen one the loss is +inf and its derivative by the margin -1. The other pair is as if alone."""
+    x, tok, gen = make(6, 300, dtype, dev, seed=53)
+    off = torch.tensor([0, 2, 4, 5, 6], dtype=torch.int32, device=dev)
+    alone = losses.preference_loss(x[4:], tok[4:], torch.arange(3, dtype=torch.int32, device=dev))
+    for row, margin, loss in ((3, math.inf, 0.0), (0, -math.inf, math.inf)):
+        y = x.clone()
+        y[row, int(tok[row])] = -math.inf
+        got = losses.preference_loss(y, tok, off)
+        assert got["margin"][0] == margin and got["pair_loss"][0] == loss and not got["pair_status"].any() and not got["row_status"].any()
+        assert got["pair_loss"][1] == alone["pair_loss"][0] and got["loss"] == alone["loss"] + loss
+        assert torch.equal(got["grad_logits"][4:], alone["grad_logits"])
+        g = torch.zeros(4, device=dev) if loss == 0 else torch.tensor([-0.1, -0.1, 0.1, 0.1], device=dev)
+        R = Rows(y[:4], tok[:4])
+        R.rel_p = torch.where(R.p > 0, R.rel_p, 0.0)
+        close(got["grad_logits"][:4], *R.gradient(g))
+        # a label that may be wrong makes a sure pair infinitely dear; a weight of 0 none
+        smooth = losses.preference_loss(y, tok, off, label_smoothing=0.1)
+        assert smooth["pair_loss"][0] == math.inf and bool(smooth["grad_logits"].isfinite().all())
+        w = losses.preference_loss(y, tok, off, pair_weight=torch.tensor([0.0, 1.0], device=dev))
+        assert w["loss"] == alone["loss"] and not w["grad_logits"][:4].any()
+
+
 @pytest.mark.parametrize("off", [[0, 3, 2], [-1, 3, 6], [0, 3, 9], [0, 2, 4, 3, 8], [0, 5, 8, 2, 3, 4, 8], [2**31 - 1, -2**31, 5]])
 def test_offsets_against_the_rules(dev, lib, off):
     x, tok, _ = make(8, 100, torch.float32, dev)
