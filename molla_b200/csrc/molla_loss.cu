@@ -581,16 +581,16 @@ template <class T, bool STATS, bool GRAD> struct Feed {
     int warp, stride;          // of the row's warps; bytes from one of its units to the next
     int row0, step;            // this cluster's rows are row0, row0 + step, ...
     int i, base; unsigned int mask;   // the row that is being fetched, and which of 32 rows are read
-    int row, before;           // the row and the one before it, -1 where there is none
+    int row;                   // -1 before the first
     const char *src; int left; // the next unit, and the bytes from there to its row's end
-    bool second;               // it is one of the row before, for the gradient
+    bool second;               // the row comes again, for its gradient
     int ahead;                 // units fetched or on their way, not given back
     int put, get, parity;      // slots
     bool more, late;
     int owed, owed_slot, owed_parity;   // copies on their way when a wait ran out
 
     __device__ __forceinline__ Feed(const LossArgs &a_, const Layout &L_, uint32_t s, uint32_t b, int w, int ws, int r0, int st)
-        : a(a_), L(L_), slots(s), bars(b), warp(w), stride(ws * UB), row0(r0), step(st), i(-1), base(-32), mask(0), row(-1), before(-1), src(nullptr), left(0), second(true),
+        : a(a_), L(L_), slots(s), bars(b), warp(w), stride(ws * UB), row0(r0), step(st), i(-1), base(-32), mask(0), row(-1), src(nullptr), left(0), second(true),
           ahead(0), put(0), get(0), parity(0), more(true), late(false), owed(0) {
         next();
         while (more && ahead < L.R) fetch();
@@ -616,22 +616,13 @@ template <class T, bool STATS, bool GRAD> struct Feed {
             if (mask >> (i - base) & 1) return row_of(i);
         }
     }
-    // From the end of one row's units to the first of another: a row for its sums, then, where units do not stay (see rows_kernel), the row before
-    // it for its gradient.
+    // From the end of one row's units to the first of another, or, where units do not stay (see rows_kernel), of the same row for its gradient.
     __device__ void next() {
         do {
-            if (STATS && GRAD && !L.resident && !second) {
-                second = true;
-                const int r = L.ahead ? before : row;
-                if (r >= 0) { start(r); continue; }
-            }
-            before = row;
-            row = before < 0 && i >= 0 ? -1 : next_row();
-            second = row < 0;
-            left = 0;
-            if (row >= 0) start(row);
-            else if (STATS && GRAD && !L.resident && L.ahead && before >= 0) start(before);
-            else { more = false; return; }
+            second = STATS && GRAD && !L.resident && !second;
+            if (!second) row = next_row();
+            if (row < 0) { more = false; return; }
+            start(row);
         } while (left <= 0);
     }
     // one more unit, where there is room
