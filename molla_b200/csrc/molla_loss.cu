@@ -273,6 +273,7 @@ constexpr int KU = UB / 512;
 template <class T> constexpr int UNIT = UB / (int)sizeof(T);   // and logits
 constexpr int MAX_WARPS = 16;      // with the one that answers
 constexpr int WAIT_TRIES = 1 << 22;   // of a bounded wait
+__device__ __forceinline__ int tries_of(const LossArgs &a) { return LOSS_KNOB(a, 256 | 512) ? 1 << 14 : WAIT_TRIES; }   // (testing build: waits that are meant to run out)
 
 // How a launch lays its rows out: C blocks of W warps a row, R units of shared memory a warp, `rows_at_once` rows
 // in flight. Nothing in a row's results depends on it: a unit is always one warp's, in the same order of additions, and
@@ -566,13 +567,13 @@ __device__ __forceinline__ bool try_for(uint32_t bar, int parity) {
         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return __all_sync(0xffffffffu, ok != 0);
 }
-__device__ __forceinline__ bool wait_for(uint32_t bar, int parity) {
+__device__ __forceinline__ bool wait_for(uint32_t bar, int parity, int tries) {
     if (try_for(bar, parity)) return true;
-    for (int i = 0; i < WAIT_TRIES; i++)
+    for (int i = 0; i < tries; i++)
         if (try_for(bar, parity)) return true;
     return false;
 }
-__device__ __forceinline__ bool wait_for(uint64_t *bar, int parity) { return wait_for(smem_u32(bar), parity); }
+__device__ __forceinline__ bool wait_for(uint64_t *bar, int parity, int tries) { return wait_for(smem_u32(bar), parity, tries); }
 
 // A warp's units of shared memory, filled in the order in which it will want them, row after row.
 template <class T, bool STATS, bool GRAD> struct Feed {
@@ -630,7 +631,8 @@ template <class T, bool STATS, bool GRAD> struct Feed {
         if (!more || ahead >= L.R) return;
         if ((threadIdx.x & 31) == 0) {
             const uint32_t to = slots + put * UB, bar = bars + put * 8, bytes = (uint32_t)min(left, UB);
-            if (!(STATS && GRAD) || L.resident) bulk_copy(to, src, bytes, bar, ANY);
+            if (LOSS_KNOB(a, 512) && warp == 0 && !second && row == a.B / 2) {   // (testing build: a copy that never comes)
+            } else if (!(STATS && GRAD) || L.resident) bulk_copy(to, src, bytes, bar, ANY);
             else if (second) bulk_copy(to, src, bytes, bar, LAST);
             else bulk_copy(to, src, bytes, bar, KEEP);
         }
@@ -644,7 +646,7 @@ template <class T, bool STATS, bool GRAD> struct Feed {
     __device__ __forceinline__ uint32_t wait(int k) {
         int s = get + k, p = parity;
         if (s >= L.R) { s -= L.R; p ^= 1; }
-        if (!late && !wait_for(bars + s * 8, p)) lose(k);
+        if (!late && !wait_for(bars + s * 8, p, tries_of(a))) lose(k);
         return slots + s * UB;
     }
     __device__ __forceinline__ uint32_t oldest() const { return slots + get * UB; }
@@ -656,6 +658,7 @@ template <class T, bool STATS, bool GRAD> struct Feed {
     }
     // a wait ran out, with the units from the k-th on still on their way: nothing more is waited for or fetched
     __device__ __forceinline__ void lose(int k = 0) {
+        if (late) return;
         late = true; more = false;
         owed = ahead - k; owed_slot = get + k; owed_parity = parity;
         if (owed_slot >= L.R) { owed_slot -= L.R; owed_parity ^= 1; }
@@ -663,7 +666,7 @@ template <class T, bool STATS, bool GRAD> struct Feed {
     // before the block's shared memory goes back, what is on its way is waited for once more
     __device__ __forceinline__ void drain() {
         for (; late && owed > 0; owed--) {
-            wait_for(bars + owed_slot * 8, owed_parity);
+            wait_for(bars + owed_slot * 8, owed_parity, tries_of(a));
             if (++owed_slot == L.R) { owed_slot = 0; owed_parity ^= 1; }
         }
     }
@@ -763,22 +766,27 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
         const int units = span.units + (span.edge() ? 1 : 0);
         // The token's logit is the first block's to fetch: where the gradient takes the logits' place nobody may write before it has been read,
         // and nobody does before it has the answer, which needs it.
-        if (!alone) {
+        if (!alone && !late) {
             if (lane == 0) mbar_expect_tx(&ctl.sums[s], (uint32_t)((max(units, L.C * L.W) + (GRAD ? 1 : 0)) * (int)sizeof(Stat)));
             if (GRAD && first && lane < L.C) put16(false, st + L.table - 1, lane, in.xt, 0.0f, 0.0f, 0.0f, &ctl.sums[s]);
         }
-        if (!late) late = !wait_for(&ctl.sums[s], (n / DEPTH) & 1);
+        if (!late) late = !wait_for(&ctl.sums[s], (n / DEPTH) & 1, tries_of(a));
+        if (late) {   // the barriers are out of step: this warp answers no more, and whoever waits for it gives up in turn
+            in.status = MOLLA_ROW_LOAD_TIMEOUT;
+            if (first && lane == 0) row_refused(a, r, in);
+            continue;
+        }
         if (GRAD && !alone) in.xt = st[L.table - 1].m;
         float M, W, depth;
         Two S;
         bool missed;
         row_stat<ENT>(st, units, c, M, S, W, depth, missed);
-        late = late || missed;   // (what was lost once has the barriers out of step)
-        if (late) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
+        if (missed) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
         Answer o;
         const RowGrad q = row_answer<ENT>(a, in, M, S, W, depth, c, o);
         __syncwarp();
-        if (GRAD || alone) {
+        if (LOSS_KNOB(a, 256) && r == a.B / 2 && rank == L.C - 1) {   // (testing build: an answer that never comes)
+        } else if (GRAD || alone) {
             if (lane == 0) {
                 ctl.share[s] = RowShare{M, c, q.A, q.H, q.token, in.token, q.A == 0.0f && q.H == 0.0f && q.token == 0.0f, 0};
                 arrive(&ctl.answered[s]);
@@ -789,8 +797,21 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
         if (first && lane == 0) row_write(a, r, in, M, S.hi, o);
         n++;
     }
-    if (late)   // what is still on its way to this block
-        for (int k = max(n - DEPTH, 0); k < n; k++) wait_for(&ctl.sums[k % DEPTH], (k / DEPTH) & 1);
+}
+
+// Rows from `first` on whose gradient a warp could not take; called when nobody else writes to them any more.
+template <class T> __device__ __noinline__ void give_up(const LossArgs &a, int first, int step) {
+    for (long long r = first; r < a.B; r += step) {
+        if (!row_read<true>(a, (int)r)) continue;
+        if ((threadIdx.x & 31) == 0) {
+            a.status[r] = MOLLA_ROW_LOAD_TIMEOUT;
+            a.logprob[r] = a.row_loss[r] = NAN;
+            if (a.entropy) a.entropy[r] = NAN;
+            if (a.kl) a.kl[r] = NAN;
+            if (a.clipped) a.clipped[r] = 0;
+        }
+        zero_row<T>((T *)a.grad + r * a.grad_stride, a.V, 0, 1);
+    }
 }
 
 template <class T, bool STATS, bool GRAD, bool ENT>
@@ -828,6 +849,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
     int n = 0;            // rows that are read
     int held = 0;         // units that stay for the gradient of the row before
     int before = -1;      // that row
+    bool cut_off = false; // a row's answer, or room for its sums, did not come in time: this warp has no part in any further row
+    int lost = -1;        // the first row whose gradient it has not taken
     for (int i = 0;; i++) {
         const int r = feed.row_of(i), from = i % 32;
         const bool last = !feed.row_ok(i);
@@ -848,10 +871,10 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
             const int s = n % DEPTH;
             const float c = __shfl_sync(0xffffffffu, mine.c, from);
             // without a gradient nobody waits for a row's answer: its table has to be free again
-            if (!GRAD && n >= DEPTH && !feed.late && !wait_for(&ctl.answered[s], (n / DEPTH + 1) & 1)) feed.lose();
-            if (!GRAD && w == 0 && lane == 0 && !alone) mbar_expect_tx(&ctl.answered[s], 16);
+            if (!GRAD && n >= DEPTH && !cut_off && !wait_for(&ctl.answered[s], (n / DEPTH + 1) & 1, tries_of(a))) { feed.lose(); cut_off = true; }
+            if (!GRAD && w == 0 && lane == 0 && !alone && !cut_off) mbar_expect_tx(&ctl.answered[s], 16);
             const Stat *st = stats + s * L.table;
-            const bool tell = lane < (GRAD ? L.C : 1);   // a lane a block that wants to know
+            const bool tell = lane < (GRAD ? L.C : 1) && !cut_off;   // a lane a block that wants to know
             for (int u = warp; u < span.units; u += warps) {
                 const uint32_t slot = feed.wait(held + units);
                 Stat o = u < span.full ? unit_stat<T, ENT, true, 1>(slot, 0, c) : unit_stat<T, ENT, false, GRAD ? 1 : 2>(slot, span.last_chunks(), c);
@@ -867,7 +890,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
             }
             // a warp without a unit says so: no row's answer may come before every warp is done with the rows before it
             __syncwarp();
-            if (alone) { if (lane == 0) arrive(&ctl.sums[s]); }
+            if (alone) { if (lane == 0 && !cut_off) arrive(&ctl.sums[s]); }
             else if (tell && warp >= span.units + (span.edge() ? 1 : 0)) put16(false, st + warp, lane, 0.0f, 0.0f, 0.0f, 0.0f, &ctl.sums[s]);
             n++;
         }
@@ -879,7 +902,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         RowShare q;
         if (STATS) {
             const int k = last || !L.ahead ? n - 1 : n - 2, s = k % DEPTH;
-            if (!feed.late && !wait_for(&ctl.answered[s], (k / DEPTH) & 1)) feed.lose();
+            if (!cut_off && !wait_for(&ctl.answered[s], (k / DEPTH) & 1, tries_of(a))) { feed.lose(); cut_off = true; lost = g; }
+            if (cut_off) continue;
             q = ctl.share[s];
         } else {
             q.M = __shfl_sync(0xffffffffu, mine.M, from); q.c = __shfl_sync(0xffffffffu, mine.c, from);
@@ -897,7 +921,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         T *at = to + warp * UNIT<T>;
         for (int u = warp; u < span.units; u += warps, at += warps * UNIT<T>) {
             const uint32_t slot = STATS && L.resident ? feed.oldest() : feed.wait(0);
-            const float A = feed.late ? NAN : q.A;
+            const float A = feed.late && !(STATS && L.resident) ? NAN : q.A;   // (units that stay are there)
             if (!q.zero) {
                 if (u < span.full && wide) unit_gradient<T, ENT, true>(slot, 0, at, true, q.M, q.c, A, q.H);
                 else unit_gradient<T, ENT, false>(slot, u < span.full ? UB / 16 : span.last_chunks(), at, wide, q.M, q.c, A, q.H);
@@ -914,9 +938,13 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
             to[edge_at] = from_f32<T>(gradient_of<T, ENT>(edge, q.M, q.c, q.A, q.H) + (edge_at == q.token - span.head ? q.token_add : 0.0f));
     }
     feed.drain();
-    if (STATS && w == 0)   // the last answers, which without a gradient nobody has waited for
-        for (int k = max(n - DEPTH, 0); k < n; k++) wait_for(&ctl.answered[k % DEPTH], (k / DEPTH) & 1);
-    if (STATS) cluster_sync();   // nobody leaves while another block has something for it
+    if (STATS) {
+        // The last answers, which without a gradient nobody has waited for; nobody leaves while another block has something for it.
+        for (int k = max(n - DEPTH, 0); k < n; k++)
+            if (!wait_for(&ctl.answered[k % DEPTH], (k / DEPTH) & 1, tries_of(a))) break;
+        cluster_sync();
+        if (GRAD && lost >= 0) give_up<T>(a, lost, step);
+    }
 }
 
 // ---- sums over rows ---------------------------------------------------------------------------------

@@ -867,3 +867,52 @@ def test_a_wait_that_runs_out_is_the_rows_status(dev, lib, V):
         assert not losses.token_logprobs_backward(x, tok, a, adv).any()
         again = losses.token_logprobs(x, tok)
     assert not again["row_status"].any() and bool(again["logprob"].isfinite().all())
+
+
+def with_knob(knob, call):
+    """The call's results in the testing build, with and without one of its switches."""
+    with capi.testing_library() as T:
+        clean = call()
+        T.molla_sample_debug_knobs(knob)
+        try:
+            late = call()
+            torch.cuda.synchronize()
+        finally:
+            T.molla_sample_debug_knobs(0)
+        again = call()
+    for a, b in zip(clean.values(), again.values()):
+        assert a is None or torch.equal(a, b)
+    return clean, late
+
+
+def check_given_up(clean, late, row, alone):
+    """Rows that were given up say so, have no numbers and a gradient of zeros; the others are what they are otherwise."""
+    gone = late["row_status"] != 0
+    assert bool(gone[row]) and (int(gone.sum()) == 1 or not alone) and not bool(gone[:row].any())
+    assert bool((late["row_status"][gone] == capi.ROW_LOAD_TIMEOUT).all()) and not bool(gone.all())
+    for name in ("logprob", "entropy", "row_loss", "kl"):
+        if late.get(name) is not None:
+            assert bool(late[name][gone].isnan().all()) and torch.equal(late[name][~gone], clean[name][~gone]), name
+    if late.get("grad_logits") is not None:
+        assert not late["grad_logits"][gone].any() and torch.equal(late["grad_logits"][~gone], clean["grad_logits"][~gone])
+    if "loss" in late:
+        assert bool(late["loss"].isnan()) and bool(clean["loss"].isfinite())
+
+
+# rows that stay in one block, in a cluster, that are read twice; alone in their blocks and several of a block
+LATE_SHAPES = [(6, 3000, torch.bfloat16), (6, 3001, torch.float32), (6, 40000, torch.float16), (6, 151936, torch.bfloat16), (3, 720896, torch.float32),
+               (900, 120000, torch.bfloat16), (5000, 3000, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("B,V,dtype", LATE_SHAPES)
+@pytest.mark.parametrize("knob", [256, 512], ids=["answer", "copy"])
+def test_an_answer_or_a_copy_that_never_comes(dev, lib, B, V, dtype, knob):
+    x, tok, gen = make(B, V, dtype, dev)
+    old, adv = normal(gen, B, dev) - 9, normal(gen, B, dev)
+    clean, late = with_knob(knob, lambda: losses.policy_loss(x, tok, old, adv, ref_logprob=old, kl_coef=0.01, entropy_coef=0.01))
+    check_given_up(clean, late, B // 2, B < 10)
+    place = lambda: (lambda y: losses.policy_loss(y, tok, old, adv, out=y))(x.clone())
+    check_given_up(*with_knob(knob, place), B // 2, B < 10)
+    if knob == 512:
+        check_given_up(*with_knob(knob, lambda: losses.policy_loss(x, tok, old, adv, want_grad=False)), B // 2, B < 10)
+        check_given_up(*with_knob(knob, lambda: losses.token_logprobs(x, tok, want_entropy=True)), B // 2, B < 10)
