@@ -273,7 +273,7 @@ constexpr int KU = UB / 512;
 template <class T> constexpr int UNIT = UB / (int)sizeof(T);   // and logits
 constexpr int MAX_WARPS = 16;      // with the one that answers
 constexpr int WAIT_TRIES = 1 << 22;   // of a bounded wait
-__device__ __forceinline__ int tries_of(const LossArgs &a) { return LOSS_KNOB(a, 256 | 512) ? 1 << 14 : WAIT_TRIES; }   // (testing build: waits that are meant to run out)
+__device__ __forceinline__ int tries_of(const LossArgs &a) { return LOSS_KNOB(a, 256 | 512 | 1024) ? 1 << 14 : WAIT_TRIES; }   // (testing build: waits that are meant to run out)
 
 // How a launch lays its rows out: C blocks of W warps a row, R units of shared memory a warp, `rows_at_once` rows
 // in flight. Nothing in a row's results depends on it: a unit is always one warp's, in the same order of additions, and
@@ -631,7 +631,7 @@ template <class T, bool STATS, bool GRAD> struct Feed {
         if (!more || ahead >= L.R) return;
         if ((threadIdx.x & 31) == 0) {
             const uint32_t to = slots + put * UB, bar = bars + put * 8, bytes = (uint32_t)min(left, UB);
-            if (LOSS_KNOB(a, 512) && warp == 0 && !second && row == a.B / 2) {   // (testing build: a copy that never comes)
+            if (LOSS_KNOB(a, second ? 1024 : 512) && warp == 0 && row == a.B / 2) {   // (testing build: a copy that never comes)
             } else if (!(STATS && GRAD) || L.resident) bulk_copy(to, src, bytes, bar, ANY);
             else if (second) bulk_copy(to, src, bytes, bar, LAST);
             else bulk_copy(to, src, bytes, bar, KEEP);
@@ -902,7 +902,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         RowShare q;
         if (STATS) {
             const int k = last || !L.ahead ? n - 1 : n - 2, s = k % DEPTH;
-            if (!cut_off && !wait_for(&ctl.answered[s], (k / DEPTH) & 1, tries_of(a))) { feed.lose(); cut_off = true; lost = g; }
+            if (!cut_off && !wait_for(&ctl.answered[s], (k / DEPTH) & 1, tries_of(a))) { feed.lose(); cut_off = true; if (lost < 0) lost = g; }
             if (cut_off) continue;
             q = ctl.share[s];
         } else {
@@ -921,8 +921,11 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         T *at = to + warp * UNIT<T>;
         for (int u = warp; u < span.units; u += warps, at += warps * UNIT<T>) {
             const uint32_t slot = STATS && L.resident ? feed.oldest() : feed.wait(0);
-            const float A = feed.late && !(STATS && L.resident) ? NAN : q.A;   // (units that stay are there)
-            if (!q.zero) {
+            const bool gone = feed.late && !(STATS && L.resident);   // (units that stay are there)
+            const float A = !STATS && gone ? NAN : q.A;
+            if (STATS && gone && !q.zero) {
+                if (lost < 0) lost = g;
+            } else if (!q.zero) {
                 if (u < span.full && wide) unit_gradient<T, ENT, true>(slot, 0, at, true, q.M, q.c, A, q.H);
                 else unit_gradient<T, ENT, false>(slot, u < span.full ? UB / 16 : span.last_chunks(), at, wide, q.M, q.c, A, q.H);
                 if (u == token_unit) {

@@ -916,3 +916,17 @@ def test_an_answer_or_a_copy_that_never_comes(dev, lib, B, V, dtype, knob):
     if knob == 512:
         check_given_up(*with_knob(knob, lambda: losses.policy_loss(x, tok, old, adv, want_grad=False)), B // 2, B < 10)
         check_given_up(*with_knob(knob, lambda: losses.token_logprobs(x, tok, want_entropy=True)), B // 2, B < 10)
+
+
+@pytest.mark.parametrize("B,V,dtype", [(3, 720896, torch.float32), (900, 120000, torch.bfloat16), (400, 120001, torch.float16), (300, 262144, torch.float32)])
+def test_a_second_copy_that_never_comes(dev, lib, B, V, dtype):
+    """Rows that are read again for their gradient: their logprobs are known by then, and are withdrawn. (Where the clip holds the row its
+    gradient is zeros without another reading: it keeps its answer.)"""
+    x, tok, gen = make(B, V, dtype, dev)
+    old, adv = normal(gen, B, dev) - 9, normal(gen, B, dev)
+    check_given_up(*with_knob(1024, lambda: losses.policy_loss(x, tok, old, adv, ref_logprob=old, kl_coef=0.01, entropy_coef=0.01)), B // 2, B < 10)
+    clean, late = with_knob(1024, lambda: (lambda y: losses.policy_loss(y, tok, old, adv, out=y))(x.clone()))
+    if clean["clipped"][B // 2]:
+        assert late["row_status"][B // 2] == 0 and not late["grad_logits"][B // 2].any()
+    else:
+        check_given_up(clean, late, B // 2, B < 10)
