@@ -402,7 +402,9 @@ int32_t molla_sample_sharded_step(void *comm, int32_t rank, int32_t world, const
  * A row with token -1 has no token: it is not read, its logprob and entropy are 0 and its gradient is zeros.
  * A row that cannot be answered says so in d_row_status (MOLLA_ROW_BAD_TOKEN, _EMPTY, _INVALID_CONFIG for
  * its temperature, _LOAD_TIMEOUT): its logprob and entropy are NaN, and so is a loss it has a part in; its
- * gradient is zeros. Logits of -inf, or of their type's lowest value, are ordinary values with p = 0; a NaN or +inf
+ * gradient is zeros. (Where a row's logits fail to come in time only when its gradient is taken from them, by the backward
+ * form or the preference loss, the gradient has NaN in the row; of the preference loss the row's status and logprob and the loss then say so as
+ * well, the pair's numbers do not.) Logits of -inf, or of their type's lowest value, are ordinary values with p = 0; a NaN or +inf
  * makes everything of its row NaN, the gradient too.
  *
  * d_grad_logits (NULL = not wanted) takes the gradient in the logits' type, rows grad_stride elements apart. It

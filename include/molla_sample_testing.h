@@ -18,7 +18,7 @@ extern "C" {
  * (nothing is withheld and nothing is left waiting): the row must come back with
  * MOLLA_ROW_LOAD_TIMEOUT, token -1 and its sampler state untouched. The losses, whose waits then give up after some
  * milliseconds: bit 256 keeps the answer for row B/2 from one of the blocks that wait for it, bit 512 never asks for a piece of row B/2,
- * bit 1024 not a second time where the row is read twice. 0 = production behaviour. */
+ * bit 1024 not a second time where the row is read twice (a preference loss's gradient among them). 0 = production behaviour. */
 void molla_sample_debug_knobs(int32_t knobs);
 
 /* When given a device buffer of B x 32 int64, later calls record clock64() stamps at the phase

@@ -631,7 +631,7 @@ template <class T, bool STATS, bool GRAD> struct Feed {
         if (!more || ahead >= L.R) return;
         if ((threadIdx.x & 31) == 0) {
             const uint32_t to = slots + put * UB, bar = bars + put * 8, bytes = (uint32_t)min(left, UB);
-            if (LOSS_KNOB(a, second ? 1024 : 512) && warp == 0 && row == a.B / 2) {   // (testing build: a copy that never comes)
+            if (LOSS_KNOB(a, second || a.follows ? 1024 : 512) && warp == 0 && row == a.B / 2) {   // (testing build: a copy that never comes)
             } else if (!(STATS && GRAD) || L.resident) bulk_copy(to, src, bytes, bar, ANY);
             else if (second) bulk_copy(to, src, bytes, bar, LAST);
             else bulk_copy(to, src, bytes, bar, KEEP);
@@ -799,18 +799,21 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
     }
 }
 
-// Rows from `first` on whose gradient a warp could not take; called when nobody else writes to them any more.
-template <class T> __device__ __noinline__ void give_up(const LossArgs &a, int first, int step) {
-    for (long long r = first; r < a.B; r += step) {
-        if (!row_read<true>(a, (int)r)) continue;
+// Rows from `first` on whose gradient a warp could not take. With STATS nobody else writes to them any more, and their gradient becomes zeros; a
+// backward pass, whose warps do not wait for one another, leaves NaN in it and says so where it has been given the places.
+template <class T, bool STATS> __device__ __noinline__ void give_up(const LossArgs &a, int first, int step) {
+    for (long long r = first; r >= 0 && r < a.B; r += step) {
+        if (!row_read<STATS>(a, (int)r)) continue;
         if ((threadIdx.x & 31) == 0) {
-            a.status[r] = MOLLA_ROW_LOAD_TIMEOUT;
-            a.logprob[r] = a.row_loss[r] = NAN;
+            if (a.status) a.status[r] = MOLLA_ROW_LOAD_TIMEOUT;
+            if (a.logprob) a.logprob[r] = NAN;
             if (a.entropy) a.entropy[r] = NAN;
             if (a.kl) a.kl[r] = NAN;
             if (a.clipped) a.clipped[r] = 0;
+            if (a.row_loss) a.row_loss[r] = NAN;
+            else if (a.loss) *a.loss = NAN;
         }
-        zero_row<T>((T *)a.grad + r * a.grad_stride, a.V, 0, 1);
+        if (STATS) zero_row<T>((T *)a.grad + r * a.grad_stride, a.V, 0, 1);
     }
 }
 
@@ -923,9 +926,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
             const uint32_t slot = STATS && L.resident ? feed.oldest() : feed.wait(0);
             const bool gone = feed.late && !(STATS && L.resident);   // (units that stay are there)
             const float A = !STATS && gone ? NAN : q.A;
-            if (STATS && gone && !q.zero) {
-                if (lost < 0) lost = g;
-            } else if (!q.zero) {
+            if (gone && !q.zero && lost < 0) lost = g;
+            if (!q.zero && !(STATS && gone)) {
                 if (u < span.full && wide) unit_gradient<T, ENT, true>(slot, 0, at, true, q.M, q.c, A, q.H);
                 else unit_gradient<T, ENT, false>(slot, u < span.full ? UB / 16 : span.last_chunks(), at, wide, q.M, q.c, A, q.H);
                 if (u == token_unit) {
@@ -946,8 +948,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 2) rows_kernel(const __grid_co
         for (int k = max(n - DEPTH, 0); k < n; k++)
             if (!wait_for(&ctl.answered[k % DEPTH], (k / DEPTH) & 1, tries_of(a))) break;
         cluster_sync();
-        if (GRAD && lost >= 0) give_up<T>(a, lost, step);
     }
+    if (GRAD && lost >= 0) give_up<T, STATS>(a, lost, !STATS && a.follows ? -step : step);
 }
 
 // ---- sums over rows ---------------------------------------------------------------------------------

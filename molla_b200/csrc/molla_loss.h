@@ -9,7 +9,7 @@ struct LossArgs {
     const void *logits; int type; long long row_stride; int B, V;
     const int *tokens; const float *temperature;
     bool follows;                // the launch is behind another one of the same call
-    // outputs of a row (any but `logprob` and `status` may be nullptr)
+    // outputs of a row (any may be nullptr, but `logprob` and `status` only in a backward pass, which touches them and `loss` where a row's logits did not come in time)
     float *logprob; float *logprob_lo; float *entropy; float *stats; unsigned int *status;   // logprob_lo: what the logprob's rounding leaves out
     // the gradient in the logits' type, or nullptr
     void *grad; long long grad_stride;

@@ -2661,6 +2661,7 @@ int32_t molla_sample_preference_loss(const void *d_logits, int32_t logits_type, 
     p.g_logprob = d_grad_logits ? g : nullptr;
     if (e == cudaSuccess) e = molla_loss_pairs(p, (cudaStream_t)stream);
     a.in_stats = stats; a.g_logprob = g; a.follows = true;
+    a.status = d_row_status; a.logprob = d_logprob; a.loss = d_loss;
     if (e == cudaSuccess && d_grad_logits) e = molla_loss_backward(a, (cudaStream_t)stream);
     return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "preference loss launch failed: %s", cudaGetErrorString(e));
 }

@@ -930,3 +930,27 @@ def test_a_second_copy_that_never_comes(dev, lib, B, V, dtype):
         assert late["row_status"][B // 2] == 0 and not late["grad_logits"][B // 2].any()
     else:
         check_given_up(clean, late, B // 2, B < 10)
+
+
+@pytest.mark.parametrize("B,V,dtype", LATE_SHAPES)
+def test_a_copy_that_never_comes_to_a_backward_pass(dev, lib, B, V, dtype):
+    """No row's gradient is silently wrong: what could not be taken is NaN, and the preference loss says which rows they are."""
+    x, tok, gen = make(B, V, dtype, dev)
+    g = normal(gen, B, dev)
+    scored = losses.token_logprobs(x, tok, want_entropy=True)
+    backward = lambda: dict(grad=losses.token_logprobs_backward(x, tok, scored, g, grad_entropy=g))
+    clean, late = with_knob(512, backward)
+    gone = late["grad"].isnan().any(1)
+    assert bool(gone[B // 2]) and not bool(gone.all()) and (int(gone.sum()) == 1 or B > 10)
+    assert torch.equal(late["grad"][~gone], clean["grad"][~gone])
+    off = torch.tensor([0, B // 3, B], dtype=torch.int32, device=dev)
+    for ref in (None, scored["logprob"]):
+        clean, late = with_knob(1024, lambda: losses.preference_loss(x, tok, off, ref_logprob=ref))
+        if not clean["grad_logits"].any():   # so sure a pair that no row's gradient is read for
+            assert ref is None and B > 10 and all(torch.equal(late[k], clean[k]) for k in clean)
+            continue
+        gone = late["grad_logits"].isnan().any(1)
+        assert bool(gone[B // 2]) and not bool(gone.all())
+        assert torch.equal(late["grad_logits"][~gone], clean["grad_logits"][~gone])
+        assert torch.equal(late["row_status"], gone.int() * capi.ROW_LOAD_TIMEOUT) and torch.equal(late["logprob"].isnan(), gone)
+        assert bool(late["loss"].isnan()) and torch.equal(late["pair_loss"], clean["pair_loss"])
