@@ -142,9 +142,8 @@ __device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in
     const float per_S = __frcp_rn(S.hi);
     o.lnS = ln_of(S.hi);
     o.lnS.lo = __fmaf_rn(S.lo, per_S, o.lnS.lo);
-    // c is log2(e)/T rounded, off by a part `off` of up to 2^-24, and with it ln S by off times the mean depth: of a logprob an error of 4e-8 at T = 1,
-    // always to the same side. An estimate of the depth that is right to a third takes it out (the logprobs' mean and standard error against 64
-    // bits before, over 128256 logits: 2e-8 and 5.5e-8).
+    // c is log2(e)/T rounded, off by a part `off` of up to 2^-24 (1.3e-8 at T = 1, 5.8e-8 at 1.1), and with it ln S by off times the mean depth: of a logprob
+    // an error of 4e-8 at T = 1, always to the same side. An estimate of the depth takes it out but for what the estimate is off by.
     const float off = (__fmaf_rn(c, in.T, -LOG2E) - LOG2E_LEFT) * LN2;
     o.lnS.lo = __fmaf_rn(off, depth, o.lnS.lo);
     const float nats = in.per_T, nats_lo = __fmaf_rn(-in.T, nats, 1.0f) * nats, dx = __fsub_rn(in.xt, M);
@@ -324,8 +323,11 @@ __device__ __forceinline__ float exp2_series(float t) {
     return p * __int_as_float(((int)n + 127) << 23);   // 0 from 2^-127 down; NaN stays in p
 }
 
-// ex2.approx is low by 5.2e-8 in the mean, alike in every binade (4 million arguments from -32 to 0), which a sum of many terms
-// keeps: uncorrected, the log ratio of a sequence of 200 rows was off by 1e-5. Its value at 0 is exact.
+// ex2.approx is low by 5.2e-8 in the mean, alike in every binade (4 million arguments from -32 to 0; by 2e-8 to 7e-8 in a sixteenth of one, which rows
+// whose exponents all lie in such a part keep the difference of), which a sum of many terms
+// keeps: uncorrected, the log ratio of a sequence of 200 rows was off by 1e-5. Its value at 0 is exact: of a unit's sum one term, its
+// largest, is left out of the correction, and a sum that is a whole number (logits that are all alike, but for those of -inf) is not corrected at all. Where
+// a unit's largest logit comes many times among others that count, its sum is high by up to 5.2e-8 of them.
 constexpr float EX2_LOW = 5.2e-8f;
 
 // 16 bytes of shared memory by their address there (pointers into it cost 64-bit arithmetic)
@@ -365,7 +367,7 @@ __device__ __forceinline__ Two warp_sum_exact(Two t) {
 __device__ __forceinline__ void put_sum(Stat &o, Two v) {
     const Two s = warp_sum_exact(v);
     o.s = s.hi;
-    o.s_lo = o.m == -INFINITY ? s.lo : __fmaf_rn(EX2_LOW, s.hi - 1.0f, s.lo);
+    o.s_lo = o.m == -INFINITY || (s.hi == rintf(s.hi) && s.lo == 0.0f) ? s.lo : __fmaf_rn(EX2_LOW, s.hi - 1.0f, s.lo);
 }
 
 // A unit's, from shared memory twice: once for its maximum, then for the sums (four of either a lane). PART: how many sums of a unit that is not full
@@ -427,9 +429,23 @@ template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) 
     return o;
 }
 
+// About how far in nats the terms of a unit's sum s lie below the largest, times their part of it: sum e (max - z) of n logits. No distribution
+// has them further than ln(n/s) on the average (nearly that where they are much alike), and the further that is from 0 the more of s belongs to a
+// few; the quarter that is left where it all does is what normal and exponential tails of any width are met by to 0.1 and 0.7 at a time (half of
+// the unit masked: 0.6). Logits that are all alike have a whole number for their sum, and lie nowhere below.
+__device__ __forceinline__ float depth_of(const Stat &o, float n) {
+    const float most = __logf(n), far = fminf(fmaxf(most - __logf(fmaxf(o.s, 1.0f)), 0.0f), most), part = __fdividef(far, most + 1e-6f);
+    const bool alike = o.s == rintf(o.s) && o.s_lo == 0.0f;
+    return alike ? 0.0f : fmaxf(o.s - 1.0f, 0.0f) * far * __fmaf_rn(-0.75f * part, part, 1.0f);
+}
+
 // All units of a row: a warp, the units in turn over the lanes, then a tree; S in two floats. `depth`: about how far in nats the logits are
-// below M on the average of the distribution; within a unit, what is not its maximum is taken to be 2.5 below it (see row_answer).
-template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int n, float c, float &M, Two &S, float &W, float &depth, bool &late) {
+// below M on the average of the distribution (see row_answer).
+template <class T, bool ENT>
+__device__ __forceinline__ void row_stat(const Stat *st, const RowSpan<T> &span, float c, float &M, Two &S, float &W, float &depth, bool &late) {
+    const int n = span.units + (span.edge() ? 1 : 0);
+    const float of_last = (float)(span.last_chunks() * Chunk<T>::N), of_edge = (float)(span.head + span.tail);
+    const auto logits_of = [&](int u) { return u < span.full ? (float)UNIT<T> : u < span.units ? of_last : of_edge; };
     const int lane = threadIdx.x & 31;
     constexpr int HELD = 3;   // units a lane that stay in registers
     Stat v[HELD];
@@ -447,17 +463,17 @@ template <bool ENT> __device__ __forceinline__ void row_stat(const Stat *st, int
     late = __any_sync(0xffffffffu, l);
     S = Two{0.0f, 0.0f};
     W = depth = 0.0f;
-    const auto add = [&](const Stat &o) {
+    const auto add = [&](const Stat &o, int u) {
         const float d = o.m == -INFINITY ? 0.0f : __fsub_rn(o.m, M);   // (a unit of -inf: sums of 0, or NaN)
         const float t = d * c, f = exp2_series(t), p = f * o.s, held = fmaxf(t, DEEP);   // (a NaN stays in f)
         const Two s = two_sum(S.hi, p);
-        depth = __fmaf_rn(f, __fmaf_rn(-held, LN2 * o.s, 2.5f * fmaxf(o.s - 1.0f, 0.0f)), depth);
+        depth = __fmaf_rn(f, __fmaf_rn(-held, LN2 * o.s, depth_of(o, logits_of(u))), depth);
         S = Two{s.hi, S.lo + (s.lo + __fmaf_rn(f, o.s_lo, __fmaf_rn(f, o.s, -p)))};
         if (ENT) W = __fmaf_rn(f, __fmaf_rn(held, o.s, o.w), W);
     };
 #pragma unroll
-    for (int k = 0; k < HELD; k++) add(v[k]);
-    for (int u = HELD * 32 + lane; u < n; u += 32) add(st[u]);
+    for (int k = 0; k < HELD; k++) add(v[k], k * 32 + lane);
+    for (int u = HELD * 32 + lane; u < n; u += 32) add(st[u], u);
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) {
         const float hi = __shfl_xor_sync(0xffffffffu, S.hi, i), lo = __shfl_xor_sync(0xffffffffu, S.lo, i);
@@ -780,7 +796,7 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
         float M, W, depth;
         Two S;
         bool missed;
-        row_stat<ENT>(st, units, c, M, S, W, depth, missed);
+        row_stat<T, ENT>(st, span, c, M, S, W, depth, missed);
         if (missed) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
         Answer o;
         const RowGrad q = row_answer<ENT>(a, in, M, S, W, depth, c, o);

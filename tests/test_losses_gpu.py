@@ -141,6 +141,69 @@ def test_strides_and_alignments(dev, lib, V, pad, shift, out_pad, out_shift, dty
     assert torch.equal(p["logprob"], got["logprob"])
 
 
+# ---- what is left of the rounding ---------------------------------------------------------------------------
+#
+# Beside a reference logprob that is the row's own, rounded to 32 bits, a sequence of one row has its log ratio in full: the logprob's
+# error is seen to 1e-13. A term of a row's sum is off by at random up to 2^-22 (its exponential) and by half a step of its exponent, for those that count 2^-23
+# or less; of many terms that is below 2^-24 of the sum as a standard error, the logarithm's 2^-25 with it. Over 2048 rows the mean
+# keeps 1/45 of that, 1.3e-9. What has one sign in all rows is larger by far where it is left in: 5e-8 of the hardware's exponential, 4e-8 of the
+# rounding of log2(e)/T, up to 2^-24 of a sum in 32 bits. MEAN is below these and above 3 x 1.3e-9 twice over.
+
+MEAN, STANDARD = 2.0**-26, 2.0**-24
+
+
+def logprob_errors(x, tok, T=None):
+    B = len(tok)
+    exact = torch.cat([Rows(x[a:a + 256], tok[a:a + 256], None if T is None else T[a:a + 256]).l for a in range(0, B, 256)])
+    ref = exact.float()
+    off = torch.arange(B + 1, dtype=torch.int32, device=x.device)
+    got = losses.preference_loss(x, tok, off, ref_logprob=ref, temperature=T, want_grad=False)
+    assert not got["row_status"].any()
+    long = losses.preference_loss(x, tok, off[[0, B // 2, B]], ref_logprob=ref, temperature=T, want_grad=False)["seq_logratio"]
+    left = exact - ref.double()
+    return got["seq_logratio"].double() - left, long.double() - left.view(2, -1).sum(1)
+
+
+def check_errors(errors, long, mean=MEAN):
+    n = len(errors) // 2
+    assert abs(float(errors.mean())) <= mean, float(errors.mean())
+    assert float(errors.std()) <= STANDARD, float(errors.std())
+    assert bool((long.abs() <= n * mean + 4 * math.sqrt(n) * STANDARD).all()), long
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,T", [(32000, None), (128256, None), (50257, 0.7), (32000, 1.3)])
+def test_errors_of_logprobs_do_not_add_up(dev, lib, V, T, dtype):
+    x, tok, gen = make(2048, V, dtype, dev, seed=59)
+    check_errors(*logprob_errors(x, tok, None if T is None else torch.full((2048,), T, device=dev)))
+
+
+@pytest.mark.parametrize("spread", [0.03, 0.3, 1.0])
+def test_errors_of_flat_rows_do_not_add_up(dev, lib, spread):
+    """Logits close to one another, at the temperature between 1/2 and 2 whose exponents are rounded most. Of a spread of 0.03 the exponents
+    have a mean of -4 x 0.03 x 1.44 / 1.1 = -0.16 and a standard deviation of 0.04: where they all lie in a sixth of a binade the exponential's errors
+    there, up to 2^-22 each, need not have the mean of a whole one, and the sum's may be as large. Of 0.3 they are spread over two binades."""
+    B, V = 2048, 32000
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(67)
+    x = spread * torch.randn((B, V), generator=gen, device=dev)
+    tok = torch.randint(0, V, (B,), generator=gen, device=dev, dtype=torch.int32)
+    check_errors(*logprob_errors(x, tok, torch.full((B,), 1.1, device=dev)), mean=2.0**-22 if spread < 0.1 else MEAN)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("masked", [False, True])
+def test_errors_of_rows_of_equal_logits_do_not_add_up(dev, lib, masked, dtype):
+    """Rows of k logits that are alike, the others -inf, at the end of the row or in between: the probabilities are 1/k."""
+    B, V = 2048, 9000
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(61)
+    k = torch.randint(700, V, (B, 1), generator=gen, device=dev)
+    place = torch.rand((B, V), generator=gen, device=dev).argsort(1) if masked else torch.arange(V, device=dev).expand(B, V)
+    x = torch.where(place < k, torch.randint(-40, 40, (B, 1), generator=gen, device=dev) / 4.0, -math.inf).to(dtype)
+    check_errors(*logprob_errors(x, place.argmin(1).to(torch.int32)))
+
+
 # ---- the policy loss -----------------------------------------------------------------------------------
 
 def policy_reference(x, tok, old, adv, w=None, ref=None, lo=0.2, hi=0.2, kl=0.0, ent=0.0, T=None, scale=1.0, grad_scale=1.0):
