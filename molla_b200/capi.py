@@ -41,7 +41,8 @@ EXPORTS = (
     "molla_sample_pick_workspace_bytes", "molla_sample_pick_rows", "molla_sample_decode_step", "molla_sample_logprobs", "molla_sample_expf", "molla_sample_logf", "molla_sample_sync",
     "molla_sample_nccl_unique_id", "molla_sample_nccl_comm_create", "molla_sample_nccl_comm_destroy",
     "molla_sample_sharded_last_error", "molla_sample_sharded_workspace_bytes", "molla_sample_sharded_step",
-    "molla_sample_token_logprobs", "molla_sample_token_logprobs_backward", "molla_sample_policy_loss",
+    "molla_sample_token_logprobs", "molla_sample_token_logprobs_backward", "molla_sample_token_logprobs_with_depth",
+    "molla_sample_token_logprobs_backward_with_depth", "molla_sample_policy_loss",
     "molla_sample_preference_workspace_bytes", "molla_sample_preference_loss",
 )
 TESTING_EXPORTS = ("molla_sample_debug_knobs", "molla_sample_debug_profile", "molla_sample_debug_topk", "molla_sample_debug_launches",
@@ -156,6 +157,10 @@ def _load(path, testing):
     L.molla_sample_token_logprobs.argtypes = block + [vp] * 5
     L.molla_sample_token_logprobs_backward.restype = i32
     L.molla_sample_token_logprobs_backward.argtypes = block + [vp] * 6 + [i64]
+    L.molla_sample_token_logprobs_with_depth.restype = i32
+    L.molla_sample_token_logprobs_with_depth.argtypes = block + [vp] * 6
+    L.molla_sample_token_logprobs_backward_with_depth.restype = i32
+    L.molla_sample_token_logprobs_backward_with_depth.argtypes = block + [vp] * 6 + [i64]
     L.molla_sample_policy_loss.restype = i32
     L.molla_sample_policy_loss.argtypes = block + [vp] * 4 + [f32] * 6 + [vp] * 8 + [i64, vp]
     L.molla_sample_preference_workspace_bytes.restype = i64

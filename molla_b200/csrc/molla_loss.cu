@@ -180,6 +180,7 @@ __device__ __forceinline__ void row_write(const LossArgs &a, int r, const RowIn 
     a.logprob[r] = status ? NAN : o.l.hi;
     if (a.logprob_lo) a.logprob_lo[r] = status ? 0.0f : o.l.lo;
     if (a.entropy) a.entropy[r] = status ? NAN : (float)H;
+    if (a.depth) a.depth[r] = status ? NAN : 0.0f - o.mean;
     if (a.stats) { a.stats[2 * r] = status ? NAN : M; a.stats[2 * r + 1] = status ? 0.0f : S; }
     if (!a.row_loss) return;
     const double bound = o.held ? (in.advantage > 0.0f ? 1.0 + (double)a.clip_high : 1.0 - (double)a.clip_low) : (double)o.ratio;
@@ -203,6 +204,7 @@ __device__ void row_idle(const LossArgs &a, int r) {
     a.logprob[r] = 0.0f;
     if (a.logprob_lo) a.logprob_lo[r] = 0.0f;
     if (a.entropy) a.entropy[r] = 0.0f;
+    if (a.depth) a.depth[r] = 0.0f;
     if (a.stats) { a.stats[2 * r] = 0.0f; a.stats[2 * r + 1] = 1.0f; }
     if (a.row_loss) a.row_loss[r] = 0.0f;
     if (a.kl) a.kl[r] = 0.0f;
@@ -539,8 +541,14 @@ __device__ __forceinline__ RowShare row_given(const LossArgs &a, int r) {
     o.token = a.tokens[r];
     o.M = a.in_stats[2 * r];
     o.c = LOG2E / T;
-    const Two lnS = ln_of(S);
-    const RowGrad q = row_grad(g, h, 1.0f / T, __frcp_rn(S), h != 0.0f ? (lnS.hi - a.in_entropy[r]) + lnS.lo : 0.0f, nats_of(o.c, T));
+    float mean = 0.0f;
+    if (h != 0.0f && a.in_depth) {
+        mean = -a.in_depth[r];
+    } else if (h != 0.0f) {   // (what rounding the entropy left out comes with it)
+        const Two lnS = ln_of(S);
+        mean = (lnS.hi - a.in_entropy[r]) + lnS.lo;
+    }
+    const RowGrad q = row_grad(g, h, 1.0f / T, __frcp_rn(S), mean, nats_of(o.c, T));
     o.A = q.A; o.H = q.H; o.token_add = q.token;
     return o;
 }
@@ -1232,7 +1240,7 @@ template <bool STATS, bool GRAD> cudaError_t launch_type(const LossArgs &a, bool
 
 }  // namespace
 
-cudaError_t molla_loss_score(const LossArgs &a, cudaStream_t st) { return launch_type<true, false>(a, a.entropy != nullptr, st); }
+cudaError_t molla_loss_score(const LossArgs &a, cudaStream_t st) { return launch_type<true, false>(a, a.entropy || a.depth, st); }
 
 cudaError_t molla_loss_backward(const LossArgs &a, cudaStream_t st) { return launch_type<false, true>(a, a.g_entropy != nullptr, st); }
 

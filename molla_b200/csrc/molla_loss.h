@@ -10,11 +10,11 @@ struct LossArgs {
     const int *tokens; const float *temperature;
     bool follows;                // the launch is behind another one of the same call
     // outputs of a row (any may be nullptr, but `logprob` and `status` only in a backward pass, which touches them and `loss` where a row's logits did not come in time)
-    float *logprob; float *logprob_lo; float *entropy; float *stats; unsigned int *status;   // logprob_lo: what the logprob's rounding leaves out
+    float *logprob; float *logprob_lo; float *entropy; float *depth; float *stats; unsigned int *status;   // logprob_lo: what the logprob's rounding leaves out; depth: sum p (max - z)
     // the gradient in the logits' type, or nullptr
     void *grad; long long grad_stride;
     // the row's derivatives, where they are given: by logprob (nullptr = the policy loss has them) and by entropy
-    const float *g_logprob; const float *g_entropy; const float *in_stats; const float *in_entropy;
+    const float *g_logprob; const float *g_entropy; const float *in_stats; const float *in_entropy; const float *in_depth;   // (one of the last two)
     // the policy loss
     const float *old_logprob; const float *advantage; const float *weight; const float *ref_logprob;
     float clip_low, clip_high, kl_coef, entropy_coef, scale, grad_scale;

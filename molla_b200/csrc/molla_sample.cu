@@ -1844,6 +1844,22 @@ int loss_gradient(LossArgs &a, void *grad, int64_t stride) {
     return MOLLA_OK;
 }
 
+int token_logprobs_backward(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V, const int32_t *d_tokens,
+                            const float *d_temperature, const float *d_stats, const float *d_entropy, const float *d_depth,
+                            const float *d_grad_logprob, const float *d_grad_entropy, void *stream, void *d_grad_logits, int64_t grad_stride) {
+    g_err[0] = 0;
+    LossArgs a = {};
+    int rc = loss_block(a, d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature);
+    if (rc != MOLLA_OK) return rc;
+    if (!d_stats || !d_grad_logprob || !d_grad_logits) return fail(MOLLA_ERR_ARGUMENT, "stats, the derivatives by the logprobs and the gradient are required%s");
+    if (d_grad_entropy && !d_entropy && !d_depth) return fail(MOLLA_ERR_ARGUMENT, "derivatives by the entropies need the entropies%s");
+    rc = loss_gradient(a, d_grad_logits, grad_stride);
+    if (rc != MOLLA_OK) return rc;
+    a.in_stats = d_stats; a.in_entropy = d_entropy; a.in_depth = d_depth; a.g_logprob = d_grad_logprob; a.g_entropy = d_grad_entropy;
+    const cudaError_t e = molla_loss_backward(a, (cudaStream_t)stream);
+    return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "gradient launch failed: %s", cudaGetErrorString(e));
+}
+
 }  // namespace
 
 extern "C" {
@@ -2566,12 +2582,20 @@ int64_t molla_sample_debug_softcap_quotients(void) {
 int32_t molla_sample_token_logprobs(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V,
                                     const int32_t *d_tokens, const float *d_temperature, void *stream, float *d_logprob,
                                     float *d_entropy, float *d_stats, uint32_t *d_row_status) {
+    return molla_sample_token_logprobs_with_depth(d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature, stream, d_logprob, d_entropy,
+                                                  nullptr, d_stats, d_row_status);
+}
+
+int32_t molla_sample_token_logprobs_with_depth(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B,
+                                               int32_t V, const int32_t *d_tokens, const float *d_temperature, void *stream,
+                                               float *d_logprob, float *d_entropy, float *d_depth, float *d_stats,
+                                               uint32_t *d_row_status) {
     g_err[0] = 0;
     LossArgs a = {};
     const int rc = loss_block(a, d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature);
     if (rc != MOLLA_OK) return rc;
     if (!d_logprob || !d_row_status) return fail(MOLLA_ERR_ARGUMENT, "logprobs and row status are required%s");
-    a.logprob = d_logprob; a.entropy = d_entropy; a.stats = d_stats; a.status = d_row_status;
+    a.logprob = d_logprob; a.entropy = d_entropy; a.depth = d_depth; a.stats = d_stats; a.status = d_row_status;
     const cudaError_t e = molla_loss_score(a, (cudaStream_t)stream);
     return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "logprob launch failed: %s", cudaGetErrorString(e));
 }
@@ -2581,17 +2605,17 @@ int32_t molla_sample_token_logprobs_backward(const void *d_logits, int32_t logit
                                              const float *d_stats, const float *d_entropy, const float *d_grad_logprob,
                                              const float *d_grad_entropy, void *stream, void *d_grad_logits,
                                              int64_t grad_stride) {
-    g_err[0] = 0;
-    LossArgs a = {};
-    int rc = loss_block(a, d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature);
-    if (rc != MOLLA_OK) return rc;
-    if (!d_stats || !d_grad_logprob || !d_grad_logits) return fail(MOLLA_ERR_ARGUMENT, "stats, the derivatives by the logprobs and the gradient are required%s");
-    if (d_grad_entropy && !d_entropy) return fail(MOLLA_ERR_ARGUMENT, "derivatives by the entropies need the entropies%s");
-    rc = loss_gradient(a, d_grad_logits, grad_stride);
-    if (rc != MOLLA_OK) return rc;
-    a.in_stats = d_stats; a.in_entropy = d_entropy; a.g_logprob = d_grad_logprob; a.g_entropy = d_grad_entropy;
-    const cudaError_t e = molla_loss_backward(a, (cudaStream_t)stream);
-    return e == cudaSuccess ? MOLLA_OK : fail(MOLLA_ERR_CUDA, "gradient launch failed: %s", cudaGetErrorString(e));
+    return token_logprobs_backward(d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature, d_stats, d_entropy, nullptr, d_grad_logprob,
+                                   d_grad_entropy, stream, d_grad_logits, grad_stride);
+}
+
+int32_t molla_sample_token_logprobs_backward_with_depth(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B,
+                                                        int32_t V, const int32_t *d_tokens, const float *d_temperature,
+                                                        const float *d_stats, const float *d_depth, const float *d_grad_logprob,
+                                                        const float *d_grad_entropy, void *stream, void *d_grad_logits,
+                                                        int64_t grad_stride) {
+    return token_logprobs_backward(d_logits, logits_type, row_stride, B, V, d_tokens, d_temperature, d_stats, nullptr, d_depth, d_grad_logprob,
+                                   d_grad_entropy, stream, d_grad_logits, grad_stride);
 }
 
 int32_t molla_sample_policy_loss(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B, int32_t V,

@@ -76,39 +76,42 @@ def _call(fn, dev: int, *args):
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, temperature: torch.Tensor | None = None,
                    want_entropy: bool = False) -> dict:
-    """Logprobs (and entropies) of one given token a row; token -1 is no token. `stats` is what
-    `token_logprobs_backward` wants."""
+    """Logprobs (and entropies) of one given token a row; token -1 is no token. `stats`, and `depth` where entropies are
+    wanted, are what `token_logprobs_backward` wants."""
     B, V, stride, kind, x, tok, dev = _block(logits, tokens)
     temp = _values("temperature", temperature, dev, B)
     status = torch.empty_like(tokens)
     stats = tokens.new_empty((B, 2), dtype=_F32)
-    logprob, entropy = stats.new_empty((2, B)).unbind(0) if want_entropy else (stats.new_empty(B), None)
+    logprob, entropy, depth = stats.new_empty((3, B)).unbind(0) if want_entropy else (stats.new_empty(B), None, None)
     if B:
-        _call(capi.lib().molla_sample_token_logprobs, dev, x, kind, stride, B, V, tok, temp, torch._C._cuda_getCurrentRawStream(dev),
-              logprob.data_ptr(), _ptr(entropy), stats.data_ptr(), status.data_ptr())
-    return dict(logprob=logprob, entropy=entropy, stats=stats, row_status=status)
+        _call(capi.lib().molla_sample_token_logprobs_with_depth, dev, x, kind, stride, B, V, tok, temp, torch._C._cuda_getCurrentRawStream(dev),
+              logprob.data_ptr(), _ptr(entropy), _ptr(depth), stats.data_ptr(), status.data_ptr())
+    return dict(logprob=logprob, entropy=entropy, depth=depth, stats=stats, row_status=status)
 
 
 def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, scored: dict, grad_logprob: torch.Tensor,
                             grad_entropy: torch.Tensor | None = None, temperature: torch.Tensor | None = None,
                             out: torch.Tensor | None = None) -> torch.Tensor:
     """The logits' gradient of a loss with these derivatives by the rows' logprobs and entropies. `scored` is
-    what `token_logprobs` returned for the same logits, tokens and temperatures. `out` may be the logits themselves."""
+    what `token_logprobs` returned for the same logits, tokens and temperatures (without its `depth` the entropies' own rounding
+    is in their part of the gradient). `out` may be the logits themselves."""
     B, V, stride, kind, x, tok, dev = _block(logits, tokens)
     temp = _values("temperature", temperature, dev, B)
     g, h = _values("grad_logprob", grad_logprob, dev, B), _values("grad_entropy", grad_entropy, dev, B)
     if grad_logprob is None:
         raise ValueError("grad_logprob is required")
-    stats, entropy = scored["stats"], scored["entropy"] if h is not None else None
-    if h is not None and entropy is None:
+    stats, depth = scored["stats"], scored.get("depth") if h is not None else None
+    entropy = scored["entropy"] if h is not None and depth is None else None
+    if h is not None and entropy is None and depth is None:
         raise ValueError("derivatives by the entropies need the entropies (want_entropy=True)")
     if stats.shape != (B, 2) or stats.get_device() != dev or stats.dtype != _F32 or not stats.is_contiguous():
         raise ValueError("the stats are of another block of logits")
-    ent = _values("entropy", entropy, dev, B)
+    of_entropy = _values("entropy", entropy, dev, B) if depth is None else _values("depth", depth, dev, B)
     out, grad_stride = _gradient(logits, stride, out)
     if B:
-        _call(capi.lib().molla_sample_token_logprobs_backward, dev, x, kind, stride, B, V, tok, temp, stats.data_ptr(), ent, g, h,
-              torch._C._cuda_getCurrentRawStream(dev), out.data_ptr(), grad_stride)
+        L = capi.lib()
+        _call(L.molla_sample_token_logprobs_backward if depth is None else L.molla_sample_token_logprobs_backward_with_depth, dev, x, kind, stride,
+              B, V, tok, temp, stats.data_ptr(), of_entropy, g, h, torch._C._cuda_getCurrentRawStream(dev), out.data_ptr(), grad_stride)
     return out
 
 

@@ -105,3 +105,18 @@ def test_the_python_side_refuses_tensors_that_do_not_fit():
         losses.policy_loss(f(2, 8), tok, f(2), f(2))
     with pytest.raises(ValueError, match="CUDA"):
         losses.preference_loss(f(2, 8), tok, torch.zeros(3, dtype=torch.int32))
+
+
+def test_the_forms_with_a_depth_refuse_what_the_others_do(lib):
+    def score_depth(logprob=P, status=P, depth=P, **k):
+        return lib.molla_sample_token_logprobs_with_depth(*block(**k), NULL, logprob, NULL, depth, NULL, status)
+
+    def backward_depth(stats=P, depth=P, g=P, h=P, grad=FAR, grad_stride=8, **k):
+        return lib.molla_sample_token_logprobs_backward_with_depth(*block(**k), stats, depth, g, h, NULL, grad, grad_stride)
+
+    for call, names in ((score_depth, ["logits", "tokens", "logprob", "status"]), (backward_depth, ["logits", "tokens", "stats", "depth", "g", "grad"])):
+        for n in names:
+            assert call(**{n: NULL}) == capi.ERR_ARGUMENT, n
+            assert capi.last_error()
+        assert call(stride=7) == capi.ERR_ARGUMENT and call(V=720897, stride=720897) == capi.ERR_VOCAB
+    assert backward_depth(grad=C.c_void_p(4096 + 4)) == capi.ERR_ARGUMENT and "overlaps" in capi.last_error()

@@ -141,6 +141,33 @@ def test_strides_and_alignments(dev, lib, V, pad, shift, out_pad, out_shift, dty
     assert torch.equal(p["logprob"], got["logprob"])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1.0, 0.6])
+def test_the_entropy_gradient_of_flat_rows(dev, lib, T, dtype):
+    """-h p (ln p + H)/T is as small as the logits are close, beside an entropy of 12. The depth between them is some 40 sums in 32 bits from
+    its terms: relatively off by 40^(1/2) 2^-24 / 3^(1/2) = 2.2e-7 as a standard error, and four times as large as a spread of the logits
+    (4.3 at 151936); 1e-6 of the gradient's norm, and each value's own roundings 3e-7. Through the entropy, off by 2.8e-7, it was 1e-5."""
+    B, V = 64, 151936
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(71)
+    x = (0.03 * torch.randn((B, V), generator=gen, device=dev)).to(dtype)
+    tok = torch.randint(0, V, (B,), generator=gen, device=dev, dtype=torch.int32)
+    temperature, zero, h = torch.full((B,), T, device=dev), torch.zeros(B, device=dev), torch.full((B,), 2.0**12, device=dev)
+    got = losses.token_logprobs(x, tok, temperature=temperature, want_entropy=True)
+    out = losses.token_logprobs_backward(x, tok, got, zero, grad_entropy=h, temperature=temperature)
+    same = losses.policy_loss(x, tok, got["logprob"], zero, entropy_coef=-(2.0**12), temperature=temperature)
+    assert torch.equal(out, same["grad_logits"]) and torch.equal(got["entropy"], same["entropy"])
+    ref = Rows(x, tok, temperature)
+    want, off = ref.gradient(zero, h)
+    close(out, want, off)
+    if dtype is torch.float32:
+        assert float((out.double() - want).norm() / want.norm()) < 2e-6
+    # callers who kept no more than the entropies
+    kept = dict(stats=got["stats"], entropy=got["entropy"])
+    close(losses.token_logprobs_backward(x, tok, kept, zero, grad_entropy=h, temperature=temperature), want,
+          off + ref.p * (h.double() * (ref.err_H + ref.H.abs() * U) / ref.T)[:, None])
+
+
 # ---- what is left of the rounding ---------------------------------------------------------------------------
 #
 # Beside a reference logprob that is the row's own, rounded to 32 bits, a sequence of one row has its log ratio in full: the logprob's
