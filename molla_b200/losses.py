@@ -14,6 +14,8 @@ temperature; greedy rows, of temperature 0, have none and are scored at one abov
 
 Loss and gradient come from one call; nothing here takes part in autograd. Calls are asynchronous on the
 current stream of the logits' device, allocate their outputs from PyTorch and keep nothing, so they can be captured in a graph.
+`out=logits.detach()` spares the gradient's memory where the logits' graph does not need their values (a linear head does not; one that
+ends in a tanh does, and its backward pass then raises, as after any operation in place).
 Rows that cannot be answered say so in `row_status` (capi.ROW_*) and turn the loss to NaN.
 """
 from __future__ import annotations
@@ -60,6 +62,7 @@ def _gradient(logits: torch.Tensor, stride: int, out):
         raise ValueError("the gradient must have the logits' shape, type and device")
     if out.numel() and (out.stride(1) != 1 and out.shape[1] > 1 or out.stride(0) < out.shape[1] and out.shape[0] > 1):
         raise ValueError("gradient rows must be contiguous and must not overlap")
+    torch.autograd.graph.increment_version(out)   # a graph that kept these values for its own backward pass has to know
     return out, max(out.stride(0), out.shape[1])
 
 

@@ -744,6 +744,33 @@ def test_autograd_agrees_on_a_head(dev, lib):
     assert float((head.grad.double() - w.grad).norm() / w.grad.norm()) < 1e-4
 
 
+def test_a_gradient_in_the_place_of_logits_that_a_graph_keeps(dev, lib):
+    """A linear head does not need its logits again: the same gradient. A tanh does: its graph refuses instead of using what is there now."""
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(73)
+    hidden, tok = torch.randn((12, 16), generator=gen, device=dev), torch.randint(0, 1000, (12,), generator=gen, device=dev, dtype=torch.int32)
+    head = (torch.randn((1000, 16), generator=gen, device=dev) * 0.3).requires_grad_()
+    old, adv, off = normal(gen, 12, dev) - 7, normal(gen, 12, dev), torch.tensor([0, 5, 12], dtype=torch.int32, device=dev)
+    calls = [lambda x, **k: losses.policy_loss(x, tok, old, adv, **k)["grad_logits"], lambda x, **k: losses.preference_loss(x, tok, off, **k)["grad_logits"],
+             lambda x, **k: losses.token_logprobs_backward(x, tok, losses.token_logprobs(x, tok), adv, **k)]
+    for call in calls:
+        grads = []
+        for place in (False, True):
+            head.grad = None
+            logits = hidden @ head.T
+            logits.backward(call(logits.detach(), **(dict(out=logits.detach()) if place else {})))
+            grads.append(head.grad.clone())
+        assert torch.equal(*grads)
+        capped = 30 * torch.tanh(hidden @ head.T / 30)
+        inner = torch.tanh(hidden @ head.T)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            inner.backward(call(inner.detach(), out=inner.detach()))
+        capped.backward(call(capped.detach(), out=capped.detach()))   # (tanh kept its own result, not the scaled one)
+        with torch.inference_mode():
+            x = torch.zeros((12, 1000), device=dev)
+            call(x, out=x)
+
+
 # ---- how it is called ------------------------------------------------------------------------------------------
 
 def everything(x, tok, off, old, ref, adv):
