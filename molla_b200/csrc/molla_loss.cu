@@ -1142,7 +1142,8 @@ Layout layout_with(int C, int W, int per_sm, int V, int size) {
 // 98 / 94, 101 / 96 (13: 98 / 96, and 40 / 45 with only 2450 rows: seven stay); backward 4, 10, 18: 162 / 151, 156 / 149, 150 / 145; policy loss with
 // its gradient, bf16, four in six blocks though the units do not stay, 15, 18, 20, 24: 228 / 196, 208 / 191, 218 / 187, 189 / 181 (16, eight in three: 198 / 202;
 // fp32, 15, 18: 158 / 168, 145 / 176); seven in four for 28, 40: 224 / 189, 202 / 187, fp32 173 / 159, 160 / 178; eleven in two, whose rounds are
-// three warps a scheduler, not four, for 63, 75 of bf16: 185 / 179, 530 / 516 (4096 rows), for 50, 16 against 15 of them: 188 / 203.
+// three warps a scheduler, not four, of bf16 63, 75: 185 / 179, 530 / 516 (4096 rows), and of 700 MB 63, 64, 65, 74, 75, 76, 77: 324 / 321, 321 / 326, 320 / 315,
+// 327 / 318, 334 / 332, 333 / 330, 336 / 330; wider rows lose by it (86, 87, 98: 346 / 348, 329 / 332, 355 / 360), and so does 50, 16 rounds against 15: 188 / 203.
 template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms) {
     const int size = (int)sizeof(T), most = (int)(((long long)V * size + UB - 1) / UB);
     int C = 1;
@@ -1170,7 +1171,7 @@ template <class T, bool STATS, bool GRAD> Layout layout_of(int B, int V, int sms
         if (share <= (size == 4 ? 28 : 41) && even(share, 7) == 7 && 40 * rounds(usual) > 23 * rounds(7)) {
             W = 7;
             per_sm = 4;
-        } else if (size == 2 && share > 41 && even(share, 11) == 11 && 10 * 3 * rounds(11) <= 9 * ((usual + 3) / 4) * rounds(usual)) {
+        } else if (size == 2 && share > 41 && share <= 80 && even(share, 11) == 11 && 10 * 3 * rounds(11) <= 9 * ((usual + 3) / 4) * rounds(usual)) {
             W = 11;
         }
     }
