@@ -1071,3 +1071,27 @@ def test_a_copy_that_never_comes_to_a_backward_pass(dev, lib, B, V, dtype):
         assert torch.equal(late["grad_logits"][~gone], clean["grad_logits"][~gone])
         assert torch.equal(late["row_status"], gone.int() * capi.ROW_LOAD_TIMEOUT) and torch.equal(late["logprob"].isnan(), gone)
         assert bool(late["loss"].isnan()) and torch.equal(late["pair_loss"], clean["pair_loss"])
+
+
+@pytest.mark.parametrize("knob", [256, 512], ids=["answer", "copy"])
+def test_clusters_of_several_rows_that_lose_one(dev, lib, knob):
+    """Four blocks a row, four rows and more a cluster: the blocks that had all they needed withdraw the row as well."""
+    B, V = 300, 262144
+    x, tok, gen = make(B, V, torch.float32, dev)
+    old, adv = normal(gen, B, dev) - 9, normal(gen, B, dev)
+    call = lambda: losses.policy_loss(x, tok, old, adv, ref_logprob=old, kl_coef=0.01, entropy_coef=0.01)
+    check_given_up(*with_knob(knob, call), B // 2, False)
+
+
+def test_room_for_sums_that_never_comes(dev, lib):
+    """Without a gradient a row's answer is wanted four rows later, when its place is to be used again: the row has its answer, rows
+    of the same block from there on have none."""
+    B, V = 20000, 3000
+    x, tok, gen = make(B, V, torch.bfloat16, dev)
+    clean, late = with_knob(256, lambda: losses.token_logprobs(x, tok, want_entropy=True))
+    gone = late["row_status"] != 0
+    assert bool(gone.any()) and not bool(gone[:B // 2 + 1].any()) and int(gone.sum()) < 40
+    assert bool((late["row_status"][gone] == capi.ROW_LOAD_TIMEOUT).all())
+    for name in ("logprob", "entropy"):
+        assert bool(late[name][gone].isnan().all()) and torch.equal(late[name][~gone], clean[name][~gone])
+    assert not losses.token_logprobs_backward(x, tok, late, torch.ones(B, device=dev))[gone].any()
