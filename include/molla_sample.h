@@ -412,6 +412,9 @@ int32_t molla_sample_sharded_step(void *comm, int32_t rank, int32_t world, const
  * output may lie in the place of an input.
  * Gradient rows whose factor is zero are zeros without the logits being read, whatever they hold.
  *
+ * The logits are what the tokens' distribution is made of: a model with a final softcap (molla_sample_decode_step applies it itself) hands in capped
+ * logits, and carries the gradient back through its cap.
+ *
  * Everything within a row is held in 32 bits or more, sums over rows in 64 bits, each in an order of its own that
  * does not depend on timing: the same call gives the same bits again. A row's logprob does not depend on
  * the other rows or their number, and is the same from all these calls (rows of the same alignment to 16 bytes). */

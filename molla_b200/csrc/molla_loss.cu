@@ -5,8 +5,9 @@
 // and for g = dL/dlogprob, h = dL/dentropy the gradient by logit j is
 //     g [j = t]/T - e_j (A + H t_j)   with  H = h/(c T T S),  A = (g - h W/(S c T))/(T S)
 // so a row needs three numbers (M, S, W) for everything. What multiplies e_j is counted in its exponent, not in x_j - M: t_j can be held at a
-// number as small as -160, where e_j is 0 whatever the temperature, so that no product of a masked logit leaves 32 bits. Differences from M are exact for the logits that matter, and
-// whatever rounding e_j has is the same in S and in the gradient, where it cancels to first order.
+// number as small as -160, where e_j is 0 whatever the temperature, so that no product of a masked logit leaves 32 bits. Differences from M are exact for the logits that matter. What
+// e_j loses to rounding at random is the same in S and in the gradient; what it loses in the mean, 5.2e-8 (EX2_LOW), is put back into S and W alone: the
+// gradient's p_j are low by that, less than half a step of 32 bits.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -32,7 +33,8 @@ constexpr float LOG2E = (float)LOG2E_64, LOG2E_LEFT = (float)(LOG2E_64 - (double
 constexpr float DEEP = -160.0f;   // where an exponent is held as a factor: 2^t is 0 below -126 (-150 with subnormals), and 0 * t stays 0 for logits of -inf
 constexpr unsigned int ROW_ERRORS = MOLLA_ROW_BAD_TOKEN | MOLLA_ROW_EMPTY | MOLLA_ROW_INVALID_CONFIG | MOLLA_ROW_LOAD_TIMEOUT;
 
-// Kernels of one call begin when the one before is about to end, and wait here until it has.
+// The later kernels of a call are launched while the one before runs, and wait here until it has ended: what is saved is their launch. (Nothing lets them begin
+// any earlier.)
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -703,16 +705,19 @@ template <class T, bool STATS, bool GRAD> struct Feed {
 //
 // A warp has a ring of shared memory to itself and fills it with bulk copies, units of 4096 bytes that only it reads: nothing
 // waits for another warp but the row's sums. Where the row fits the rings of its cluster (resident) it is read from memory once: the units stay
-// until the gradient has been taken from them; else they come a second time, out of L2. The sums of a row come before the gradient of the
-// row before it, whose answer arrives meanwhile, so that nobody waits for an answer.
+// until the gradient has been taken from them; else they come a second time, out of L2. Where the rings hold two rows (ahead: up to 8000 logits of 16
+// bits, 4000 of 32, a block) the sums of a row come before the gradient of the row before it, whose answer arrives meanwhile; all others wait, between a
+// row's sums and its gradient, for the row's answer, with the next copies on their way where a warp has two units or more.
 //
 // The sums of all units go to every block that waits for the row's answer; one warp there does nothing but put them together and answer; it has fetched
 // the rows' inputs beforehand. (As a part of one of the ordinary warps' work, between two barriers, that took 12 of 29 thousand cycles a row.)
 //
-// The least a call can take is one read of the logits and one write of the gradient. bf16 rows are bounded by instructions first: one exponential a logit
-// for the sums and one for the gradient, at 16 a cycle and SM, among nineteen instructions a logit (106 M of a warp for 1184 x 151936, issue slots
-// 60 % busy; 4096 x 151936 in 530 us, 73 % of what a copy of those bytes takes; their logprobs alone, 8288 x 128256, in 381 us, 86 %); fp32 rows and the backward
-// pass by HBM and by what the second read finds in L2 (2072 x 128256 fp32 402 us, 82 %; backward 3600 x 128256 bf16 309 us, 92 %).
+// The least a call can take is one read of the logits and one write of the gradient. In bf16 rows with a gradient nothing is at its limit: nineteen instructions a
+// logit (106 M of a warp for 1184 x 151936) keep the issue slots 60 % busy, two exponentials a logit half of their unit, DRAM is at 73 % of the copy rate
+// (4096 x 151936 in 521 us); the warps wait for the row's answer, for one another's turn at the exponentials and for second reads that miss L2 (a quarter).
+// Their logprobs alone, 8288 x 128256, take 381 us, 86 %; fp32 rows and the backward pass are bounded by HBM and by what the second read
+// finds in L2 (2072 x 128256 fp32 402 us, 82 %; backward 3600 x 128256 bf16 309 us, 92 %). fp16 takes what bf16 takes (4096 x 151936 522 us). A gradient whose rows begin
+// elsewhere within 16 bytes than their logits is stored an element at a time: backward 2048 x 128256 bf16 187 us, one element off 578; policy 231 / 503; fp32 356 / 405.
 constexpr int DEPTH = 4;   // rows whose sums may be on their way
 
 struct alignas(16) Control {
@@ -1123,7 +1128,8 @@ Layout layout_with(int C, int W, int per_sm, int V, int size) {
     return L;
 }
 
-// Long rows have 13 warps in two blocks an SM, with two units of shared memory each; rows (or a block's part of them) of up to 18 units as many
+// Long rows have 13 warps in two blocks an SM, with two units of shared memory each (one where the tables of sums leave no more, and then
+// nothing is on its way while the warp works: fp32 rows of 125 to 133, 150 to 159, 197 to 212 and 250 to 262 thousand logits, 16-bit ones from 250 thousand); rows (or a block's part of them) of up to 18 units as many
 // warps as leave two units to a warp, in as many more blocks an SM, so that they stay in shared memory; rows of up to 4 units a warp a unit.
 // Policy loss with its gradient, us, in 2 / 3 / 5 / 6 / 10 blocks an SM: 4096 x 32000 bf16 146 / 124 / 126 / 126 / 135, 8192 x 50304 bf16
 // 357 / 433 / - / - / -, 16384 x 8000 bf16 296 / 228 / 165 / 165 / 168, 32768 x 2000 bf16 554 / 386 / 259 / 222 / 161.

@@ -7,7 +7,9 @@ They start where the sampling calls stop. A rollout's tokens and old logprobs:
     old = losses.token_logprobs(logits, out["tokens"], temperature=params["temperature"])["logprob"]
 
 (`chosen_logprob` is of the logits as the model gave them; rows drawn at a temperature have the logprobs of that
-temperature; greedy rows, of temperature 0, have none and are scored at one above it.) A training step, for logits that an autograd graph made:
+temperature; greedy rows, of temperature 0, have none and are scored at one above it. These are of the whole distribution: where top-k, top-p,
+min-p, penalties or biases took part in the draw, the token was drawn from what they left. A final softcap is applied before
+the logits come here: a decode step does so itself (`final_softcap`), nothing here does.) A training step, for logits that an autograd graph made:
 
     got = losses.policy_loss(logits.detach(), tokens, old, advantage, weight=mask, temperature=temperature, scale=1 / n_tokens)
     logits.backward(got["grad_logits"])
