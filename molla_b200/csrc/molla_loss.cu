@@ -433,23 +433,29 @@ template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) 
     return o;
 }
 
-// About how far in nats the terms of a unit's sum s lie below the largest, times their part of it: sum e (max - z) of n logits. No distribution
-// has them further than ln(n/s) on the average (nearly that where they are much alike), and the further that is from 0 the more of s belongs to a
-// few; the quarter that is left where it all does is what normal and exponential tails of any width are met by to 0.1 and 0.7 at a time (half of
-// the unit masked: 0.6). Logits that are all alike have a whole number for their sum, and lie nowhere below.
-__device__ __forceinline__ float depth_of(const Stat &o, float n) {
-    const float most = __logf(n), far = fminf(fmaxf(most - __logf(fmaxf(o.s, 1.0f)), 0.0f), most), part = __fdividef(far, most + 1e-6f);
-    const bool alike = o.s == rintf(o.s) && o.s_lo == 0.0f;
-    return alike ? 0.0f : fmaxf(o.s - 1.0f, 0.0f) * far * __fmaf_rn(-0.75f * part, part, 1.0f);
+// A number n of logits: ln n, and -3/4 of its square's inverse. (Worked out while the sums are awaited.)
+struct Count { float ln, curve; };
+__device__ __forceinline__ Count count_of(int n) {
+    const float ln = __logf((float)n);
+    return Count{ln, n > 1 ? -__fdividef(0.75f, ln * ln) : 0.0f};
+}
+// About sum e (max - z) in nats over a unit's n logits, of a sum s: s - 1 times how far below the largest the others lie. No distribution has them
+// further than ln(n/s) on the average: nearly that where they are much alike, less the more of s belongs to a few. With 1 - 3/4 (ln(n/s) / ln n)^2 of it
+// normal tails of any width are met to 0.2, exponential ones to 0.7, a unit that is half masked to 0.6. Logits that are all alike have
+// a whole number for their sum, and lie nowhere below.
+__device__ __forceinline__ float depth_of(const Stat &o, const Count &n) {
+    const float far = n.ln - __logf(o.s);
+    return o.s <= 1.0f || (o.s == rintf(o.s) && o.s_lo == 0.0f) ? 0.0f : (o.s - 1.0f) * far * __fmaf_rn(n.curve * far, far, 1.0f);
 }
 
 // All units of a row: a warp, the units in turn over the lanes, then a tree; S in two floats. `depth`: about how far in nats the logits are
 // below M on the average of the distribution (see row_answer).
 template <class T, bool ENT>
-__device__ __forceinline__ void row_stat(const Stat *st, const RowSpan<T> &span, float c, float &M, Two &S, float &W, float &depth, bool &late) {
+__device__ __forceinline__ void row_stat(const Stat *st, const RowSpan<T> &span, const Count &of_last, const Count &of_edge, float c, float &M, Two &S,
+                                         float &W, float &depth, bool &late) {
     const int n = span.units + (span.edge() ? 1 : 0);
-    const float of_last = (float)(span.last_chunks() * Chunk<T>::N), of_edge = (float)(span.head + span.tail);
-    const auto logits_of = [&](int u) { return u < span.full ? (float)UNIT<T> : u < span.units ? of_last : of_edge; };
+    constexpr float LN_UNIT = sizeof(T) == 4 ? 6.93147181f : 7.62461899f;   // ln 1024, ln 2048
+    const auto count = [&](int u) { return u < span.full ? Count{LN_UNIT, -0.75f / (LN_UNIT * LN_UNIT)} : u < span.units ? of_last : of_edge; };
     const int lane = threadIdx.x & 31;
     constexpr int HELD = 3;   // units a lane that stay in registers
     Stat v[HELD];
@@ -471,7 +477,7 @@ __device__ __forceinline__ void row_stat(const Stat *st, const RowSpan<T> &span,
         const float d = o.m == -INFINITY ? 0.0f : __fsub_rn(o.m, M);   // (a unit of -inf: sums of 0, or NaN)
         const float t = d * c, f = exp2_series(t), p = f * o.s, held = fmaxf(t, DEEP);   // (a NaN stays in f)
         const Two s = two_sum(S.hi, p);
-        depth = __fmaf_rn(f, __fmaf_rn(-held, LN2 * o.s, depth_of(o, logits_of(u))), depth);
+        depth = __fmaf_rn(f, __fmaf_rn(-held, LN2 * o.s, depth_of(o, count(u))), depth);
         S = Two{s.hi, S.lo + (s.lo + __fmaf_rn(f, o.s_lo, __fmaf_rn(f, o.s, -p)))};
         if (ENT) W = __fmaf_rn(f, __fmaf_rn(held, o.s, o.w), W);
     };
@@ -799,6 +805,7 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
             if (lane == 0) mbar_expect_tx(&ctl.sums[s], (uint32_t)((max(units, L.C * L.W) + (GRAD ? 1 : 0)) * (int)sizeof(Stat)));
             if (GRAD && first && lane < L.C) put16(false, st + L.table - 1, lane, in.xt, 0.0f, 0.0f, 0.0f, &ctl.sums[s]);
         }
+        const Count of_last = count_of(span.last_chunks() * Chunk<T>::N), of_edge = count_of(span.head + span.tail);   // (where there are any)
         if (!late) late = !wait_for(&ctl.sums[s], (n / DEPTH) & 1, tries_of(a));
         if (late) {   // the barriers are out of step: this warp answers no more, and whoever waits for it gives up in turn
             in.status = MOLLA_ROW_LOAD_TIMEOUT;
@@ -809,7 +816,7 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
         float M, W, depth;
         Two S;
         bool missed;
-        row_stat<T, ENT>(st, span, c, M, S, W, depth, missed);
+        row_stat<T, ENT>(st, span, of_last, of_edge, c, M, S, W, depth, missed);
         if (missed) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
         Answer o;
         const RowGrad q = row_answer<ENT>(a, in, M, S, W, depth, c, o);
