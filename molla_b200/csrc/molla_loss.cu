@@ -5,9 +5,9 @@
 // and for g = dL/dlogprob, h = dL/dentropy the gradient by logit j is
 //     g [j = t]/T - e_j (A + H t_j)   with  H = h/(c T T S),  A = (g - h W/(S c T))/(T S)
 // so a row needs three numbers (M, S, W) for everything. What multiplies e_j is counted in its exponent, not in x_j - M: t_j can be held at a
-// number as small as -160, where e_j is 0 whatever the temperature, so that no product of a masked logit leaves 32 bits. Differences from M are exact for the logits that matter. What
-// e_j loses to rounding at random is the same in S and in the gradient; what it loses in the mean, 5.2e-8 (EX2_LOW), is put back into S and W alone: the
-// gradient's p_j are low by that, less than half a step of 32 bits.
+// number as small as -160, where e_j is 0 whatever the temperature, so that no product of a masked logit leaves 32 bits. Differences from M are exact for the logits that matter. Whatever
+// rounding e_j has is the same in S, in W and in the gradient, where it cancels to first order; what it has in the mean is known (EX2_LOW, rounding_of), kept
+// beside S and counted in ln S alone.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -139,15 +139,11 @@ __device__ __forceinline__ float exp_less_line(float q, float &less_one) {
 struct Answer { unsigned int status; Two l, lnS; float mean, ratio, kl; bool held; };
 
 template <bool ENT>
-__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in, float M, Two S, float W, float depth, float c, Answer &o) {
+__device__ __forceinline__ RowGrad row_answer(const LossArgs &a, const RowIn &in, float M, Two S, float W, float c, Answer &o) {
     o.status = in.status | (M == -INFINITY && S.hi == 0.0f && !in.status ? MOLLA_ROW_EMPTY : 0u);
     const float per_S = __frcp_rn(S.hi);
     o.lnS = ln_of(S.hi);
     o.lnS.lo = __fmaf_rn(S.lo, per_S, o.lnS.lo);
-    // c is log2(e)/T rounded, off by a part `off` of up to 2^-24 (1.3e-8 at T = 1, 5.8e-8 at 1.1), and with it ln S by off times the mean depth: of a logprob
-    // an error of 4e-8 at T = 1, always to the same side. An estimate of the depth takes it out but for what the estimate is off by.
-    const float off = (__fmaf_rn(c, in.T, -LOG2E) - LOG2E_LEFT) * LN2;
-    o.lnS.lo = __fmaf_rn(off, depth, o.lnS.lo);
     const float nats = in.per_T, nats_lo = __fmaf_rn(-in.T, nats, 1.0f) * nats, dx = __fsub_rn(in.xt, M);
     const float per_cT = ENT ? nats_of(c, in.T) : 0.0f;
     o.mean = ENT ? W * per_S * per_cT : 0.0f;
@@ -358,20 +354,30 @@ template <> __device__ __forceinline__ float lds_element<__half>(uint32_t at) { 
 struct Stat { float m, s, w, s_lo; };
 constexpr float LATE = -1.0f;
 
-// The sum over a warp of values from 0 to 64, to 2^-38 each: in integers of 2^-16 and, for what that leaves, of 2^-38 (the bits that an addition
-// to 192, or to 1.5 2^-15, ends in), which add up exactly in whatever order. (A tree of 32-bit sums loses what is below half a step of the
-// largest value, always downwards: 5e-8 of a unit, which the log ratio of a long sequence adds up.) A NaN stays.
-__device__ __forceinline__ Two warp_sum_exact(Two t) {
-    const float v = t.hi, high = __fadd_rn(v, 192.0f), left = __fadd_rn(__fsub_rn(v, __fsub_rn(high, 192.0f)), t.lo), low = __fadd_rn(left, 1.5f / 32768.0f);
-    const int A = __reduce_add_sync(0xffffffffu, __float_as_int(high) - __float_as_int(192.0f));
-    const int B = __reduce_add_sync(0xffffffffu, __float_as_int(low) - __float_as_int(1.5f / 32768.0f));
-    const Two s = two_sum((float)(A >> 8) * (1.0f / 256.0f), __fmaf_rn((float)B, 1.0f / 274877906944.0f, (float)(A & 255) * (1.0f / 65536.0f)));
-    return __any_sync(0xffffffffu, !(v <= 64.0f)) ? Two{NAN, 0.0f} : s;
+// A lane's sum of values from 0 to 16, up to 64 altogether, without loss: 128 and what is above it in one float, whose last bit is 2^-16, and what each
+// addition to it rounds off, up to 2^-17, in another.
+struct Sum {
+    float high = 128.0f, low = 0.0f;
+    __device__ __forceinline__ void add(float v) {
+        const float h = __fadd_rn(high, v);
+        low = low + __fsub_rn(v, __fsub_rn(h, high));
+        high = h;
+    }
+};
+// Those of a warp: in integers of 2^-16 and, of what is left (up to four times 2^-17), of 2^-36 (the bits that an addition to 1.5 2^-13 ends in), which add
+// up exactly in whatever order. (A tree of 32-bit sums loses what is below half a step of the largest value, always downwards: 5e-8 of a unit,
+// which the log ratio of a long sequence adds up.) A NaN stays.
+__device__ __forceinline__ Two warp_sum_exact(const Sum &t) {
+    const float low = __fadd_rn(t.low, 1.5f / 8192.0f);
+    const int A = __reduce_add_sync(0xffffffffu, __float_as_int(t.high) - __float_as_int(128.0f));
+    const int B = __reduce_add_sync(0xffffffffu, __float_as_int(low) - __float_as_int(1.5f / 8192.0f));
+    const Two s = two_sum((float)(A >> 8) * (1.0f / 256.0f), __fmaf_rn((float)B, 1.0f / 68719476736.0f, (float)(A & 255) * (1.0f / 65536.0f)));
+    return __any_sync(0xffffffffu, !(t.high < 256.0f)) ? Two{NAN, 0.0f} : s;
 }
-__device__ __forceinline__ void put_sum(Stat &o, Two v) {
-    const Two s = warp_sum_exact(v);
+__device__ __forceinline__ void put_sum(Stat &o, const Sum &t) {
+    const Two s = warp_sum_exact(t);
     o.s = s.hi;
-    o.s_lo = o.m == -INFINITY || (s.hi == rintf(s.hi) && s.lo == 0.0f) ? s.lo : __fmaf_rn(EX2_LOW, s.hi - 1.0f, s.lo);
+    o.s_lo = s.lo;
 }
 
 // A unit's, from shared memory twice: once for its maximum, then for the sums (four of either a lane). PART: how many sums of a unit that is not full
@@ -394,7 +400,7 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
     // it would lose up to half a step, and what is smaller than that altogether (the logprobs of 128256 bf16 logits were low by 1.5e-8 on the
     // average, with a standard error of 3.8e-8; so they are right to 1e-9 on the average, with 2.7e-8, for 1 % of the time).
     constexpr int CHUNKS = 16 / Chunk<T>::N;
-    Two sum{0.0f, 0.0f};
+    Sum sum;
     float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll(FULL ? KU / 2 / CHUNKS : PART)
     for (int k0 = 0; k0 < KU; k0 += CHUNKS) {
@@ -411,15 +417,11 @@ __device__ __forceinline__ Stat unit_stat(uint32_t slot, int chunks, float c) {
                     if (ENT) w[i & 3] = __fmaf_rn(e, fmaxf(t, DEEP), w[i & 3]);
                 }
             }
-        const Two next = two_sum(sum.hi, (s[0] + s[1]) + (s[2] + s[3]));
-        sum = Two{next.hi, sum.lo + next.lo};
+        sum.add((s[0] + s[1]) + (s[2] + s[3]));
     }
     put_sum(o, sum);
     o.w = 0.0f;
-    if (ENT) {
-        const float ws = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
-        o.w = __fmaf_rn(EX2_LOW, ws, ws);
-    }
+    if (ENT) o.w = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
     return o;
 }
 
@@ -428,31 +430,43 @@ template <bool ENT> __device__ __forceinline__ Stat edge_stat(float x, float c) 
     Stat o;
     o.m = warp_max(x);
     const float m = o.m == -INFINITY ? 0.0f : o.m, t = __fsub_rn(x, m) * c, e = ex2(t);
-    put_sum(o, Two{e, 0.0f});
+    Sum sum;
+    sum.add(e);
+    put_sum(o, sum);
     o.w = ENT ? warp_sum(e * fmaxf(t, DEEP)) : 0.0f;
     return o;
 }
 
-// A number n of logits: ln n, and -3/4 of its square's inverse. (Worked out while the sums are awaited.)
+// A number n of logits: ln n, and -3/4 of its square's inverse.
 struct Count { float ln, curve; };
 __device__ __forceinline__ Count count_of(int n) {
     const float ln = __logf((float)n);
     return Count{ln, n > 1 ? -__fdividef(0.75f, ln * ln) : 0.0f};
 }
-// About sum e (max - z) in nats over a unit's n logits, of a sum s: s - 1 times how far below the largest the others lie. No distribution has them
-// further than ln(n/s) on the average: nearly that where they are much alike, less the more of s belongs to a few. With 1 - 3/4 (ln(n/s) / ln n)^2 of it
-// normal tails of any width are met to 0.2, exponential ones to 0.7, a unit that is half masked to 0.6. Logits that are all alike have
-// a whole number for their sum, and lie nowhere below.
-__device__ __forceinline__ float depth_of(const Stat &o, const Count &n) {
-    const float far = n.ln - __logf(o.s);
-    return o.s <= 1.0f || (o.s == rintf(o.s) && o.s_lo == 0.0f) ? 0.0f : (o.s - 1.0f) * far * __fmaf_rn(n.curve * far, far, 1.0f);
+// ln s to 0.03 for s from 1 to 4096: its bits are its logarithm, but for a curve. (None of this runs where the exponentials do.)
+__device__ __forceinline__ float about_ln(float s) {
+    const float bits = __int_as_float(0x4b000000 | (__float_as_int(s) >> 8));
+    return __fmaf_rn(__fsub_rn(bits, 8388608.0f + 0x3f8000), LN2 / 32768.0f, 0.03f);
+}
+// What a unit's sum s of n logits lacks: the part EX2_LOW of all but its largest term, and `off` (rounding_of) of sum e (max - z). That is about
+// s - 1 times how far in nats the others lie below the largest. No distribution has them further than ln(n/s) on the average: nearly that where they are much
+// alike, less the more of s belongs to a few. With 1 - 3/4 (ln(n/s) / ln n)^2 of it normal tails of any width are met to 0.2, exponential
+// ones to 0.7, a unit that is half masked to 0.6. Logits that are all alike have a whole number for their sum, which lacks nothing.
+__device__ __forceinline__ float lacks(const Stat &o, const Count &n, float off) {
+    const float far = n.ln - about_ln(o.s), whole = __fsub_rn(__fadd_rn(o.s, 12582912.0f), 12582912.0f);
+    const float by = __fmaf_rn(off * far, __fmaf_rn(n.curve * far, far, 1.0f), EX2_LOW);
+    return whole == o.s && o.s_lo == 0.0f ? 0.0f : (o.s - 1.0f) * by;
 }
 
-// All units of a row: a warp, the units in turn over the lanes, then a tree; S in two floats. `depth`: about how far in nats the logits are
-// below M on the average of the distribution (see row_answer).
+// c is log2(e)/T rounded: off by this part of it, up to 2^-24 (1.3e-8 at T = 1, 5.8e-8 at 1.1).
+__device__ __forceinline__ float rounding_of(float c, float T) { return (__fmaf_rn(c, T, -LOG2E) - LOG2E_LEFT) * LN2; }
+
+// All units of a row: a warp, the units in turn over the lanes, then a tree; S in two floats: the sum of what has been added up, and what that lost or lacks.
+// What is `off` in c (rounding_of) puts ln S off by that times how far in nats the logits are below M on the average of the distribution: of a logprob an
+// error of 4e-8 at T = 1, always to the same side.
 template <class T, bool ENT>
-__device__ __forceinline__ void row_stat(const Stat *st, const RowSpan<T> &span, const Count &of_last, const Count &of_edge, float c, float &M, Two &S,
-                                         float &W, float &depth, bool &late) {
+__device__ __forceinline__ void row_stat(const Stat *st, const RowSpan<T> &span, const Count &of_last, const Count &of_edge, float c, float off, float &M,
+                                         Two &S, float &W, bool &late) {
     const int n = span.units + (span.edge() ? 1 : 0);
     constexpr float LN_UNIT = sizeof(T) == 4 ? 6.93147181f : 7.62461899f;   // ln 1024, ln 2048
     const auto count = [&](int u) { return u < span.full ? Count{LN_UNIT, -0.75f / (LN_UNIT * LN_UNIT)} : u < span.units ? of_last : of_edge; };
@@ -464,6 +478,7 @@ __device__ __forceinline__ void row_stat(const Stat *st, const RowSpan<T> &span,
 #pragma unroll
     for (int k = 0; k < HELD; k++) {
         v[k] = Stat{-INFINITY, 0.0f, 0.0f, 0.0f};
+        if (k > 0 && k * 32 >= n) continue;
         if (k * 32 + lane < n) v[k] = st[k * 32 + lane];
         m = fmaxf(m, v[k].m);
         l |= v[k].s_lo == LATE;
@@ -472,27 +487,25 @@ __device__ __forceinline__ void row_stat(const Stat *st, const RowSpan<T> &span,
     M = warp_max(m);
     late = __any_sync(0xffffffffu, l);
     S = Two{0.0f, 0.0f};
-    W = depth = 0.0f;
+    W = 0.0f;
     const auto add = [&](const Stat &o, int u) {
         const float d = o.m == -INFINITY ? 0.0f : __fsub_rn(o.m, M);   // (a unit of -inf: sums of 0, or NaN)
         const float t = d * c, f = exp2_series(t), p = f * o.s, held = fmaxf(t, DEEP);   // (a NaN stays in f)
         const Two s = two_sum(S.hi, p);
-        depth = __fmaf_rn(f, __fmaf_rn(-held, LN2 * o.s, depth_of(o, count(u))), depth);
-        S = Two{s.hi, S.lo + (s.lo + __fmaf_rn(f, o.s_lo, __fmaf_rn(f, o.s, -p)))};
+        const float left = __fmaf_rn(off * LN2 * held, -o.s, o.s_lo + lacks(o, count(u), off));
+        S = Two{s.hi, S.lo + (s.lo + __fmaf_rn(f, left, __fmaf_rn(f, o.s, -p)))};
         if (ENT) W = __fmaf_rn(f, __fmaf_rn(held, o.s, o.w), W);
     };
 #pragma unroll
-    for (int k = 0; k < HELD; k++) add(v[k], k * 32 + lane);
+    for (int k = 0; k < HELD; k++)
+        if (k == 0 || k * 32 < n) add(v[k], k * 32 + lane);
     for (int u = HELD * 32 + lane; u < n; u += 32) add(st[u], u);
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) {
         const float hi = __shfl_xor_sync(0xffffffffu, S.hi, i), lo = __shfl_xor_sync(0xffffffffu, S.lo, i);
         const Two s = two_sum(S.hi, hi);
         S = Two{s.hi, (S.lo + lo) + s.lo};
-        depth += __shfl_xor_sync(0xffffffffu, depth, i);
     }
-    S = two_sum(S.hi, S.lo);
-    depth *= __frcp_rn(S.hi);
     if (ENT) W = warp_sum(W);
 }
 
@@ -767,6 +780,8 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
     const bool alone = L.C == 1, first = rank == 0;
     bool late = false;
     int n = 0;   // rows that are read
+    int head = -1, tail = -1;   // of the row before, and the logits of its last units
+    Count of_last{}, of_edge{};
     RowIn mine = {};
     unsigned int mask = 0;
     for (int i = 0; (long long)row0 + (long long)i * step < a.B; i++) {
@@ -805,7 +820,11 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
             if (lane == 0) mbar_expect_tx(&ctl.sums[s], (uint32_t)((max(units, L.C * L.W) + (GRAD ? 1 : 0)) * (int)sizeof(Stat)));
             if (GRAD && first && lane < L.C) put16(false, st + L.table - 1, lane, in.xt, 0.0f, 0.0f, 0.0f, &ctl.sums[s]);
         }
-        const Count of_last = count_of(span.last_chunks() * Chunk<T>::N), of_edge = count_of(span.head + span.tail);   // (where there are any)
+        if (span.head != head || span.tail != tail) {   // (seldom: the rows' sizes are alike where they begin alike)
+            head = span.head; tail = span.tail;
+            of_last = count_of(span.last_chunks() * Chunk<T>::N); of_edge = count_of(head + tail);
+        }
+        const float off = rounding_of(c, in.T);
         if (!late) late = !wait_for(&ctl.sums[s], (n / DEPTH) & 1, tries_of(a));
         if (late) {   // the barriers are out of step: this warp answers no more, and whoever waits for it gives up in turn
             in.status = MOLLA_ROW_LOAD_TIMEOUT;
@@ -813,13 +832,13 @@ __device__ __forceinline__ void answer_rows(const LossArgs &a, const Layout &L, 
             continue;
         }
         if (GRAD && !alone) in.xt = st[L.table - 1].m;
-        float M, W, depth;
+        float M, W;
         Two S;
         bool missed;
-        row_stat<T, ENT>(st, span, of_last, of_edge, c, M, S, W, depth, missed);
+        row_stat<T, ENT>(st, span, of_last, of_edge, c, off, M, S, W, missed);
         if (missed) in.status |= MOLLA_ROW_LOAD_TIMEOUT;
         Answer o;
-        const RowGrad q = row_answer<ENT>(a, in, M, S, W, depth, c, o);
+        const RowGrad q = row_answer<ENT>(a, in, M, S, W, c, o);
         __syncwarp();
         if (LOSS_KNOB(a, 256) && r == a.B / 2 && rank == L.C - 1) {   // (testing build: an answer that never comes)
         } else if (GRAD || alone) {
