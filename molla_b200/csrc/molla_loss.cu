@@ -732,11 +732,11 @@ template <class T, bool STATS, bool GRAD> struct Feed {
 // the rows' inputs beforehand. (As a part of one of the ordinary warps' work, between two barriers, that took 12 of 29 thousand cycles a row.)
 //
 // The least a call can take is one read of the logits and one write of the gradient. In bf16 rows with a gradient nothing is at its limit: nineteen instructions a
-// logit (106 M of a warp for 1184 x 151936) keep the issue slots 60 % busy, two exponentials a logit half of their unit, DRAM is at 73 % of the copy rate
-// (4096 x 151936 in 521 us); the warps wait for the row's answer, for one another's turn at the exponentials and for second reads that miss L2 (a quarter).
-// Their logprobs alone, 8288 x 128256, take 381 us, 86 %; fp32 rows and the backward pass are bounded by HBM and by what the second read
-// finds in L2 (2072 x 128256 fp32 402 us, 82 %; backward 3600 x 128256 bf16 309 us, 92 %). fp16 takes what bf16 takes (4096 x 151936 522 us). A gradient whose rows begin
-// elsewhere within 16 bytes than their logits is stored an element at a time: backward 2048 x 128256 bf16 187 us, one element off 578; policy 231 / 503; fp32 356 / 405.
+// logit (104 M of a warp for 1184 x 151936) keep the issue slots 62 % busy, two exponentials a logit half of their unit, DRAM is at 74 % of the copy rate
+// (4096 x 151936 in 517 us); the warps wait for the row's answer, for one another's turn at the exponentials and for second reads that miss L2 (a quarter).
+// Their logprobs alone, 8288 x 128256, take 371 us, 89 %, with the issue slots 73 % busy; fp32 rows and the backward pass are bounded by HBM and by what the second read
+// finds in L2 (2072 x 128256 fp32 404 us, 81 %; backward 3600 x 128256 bf16 316 us, 90 %). fp16 takes what bf16 takes (4096 x 151936 514 us). A gradient whose rows begin
+// elsewhere within 16 bytes than their logits is stored an element at a time: backward 2048 x 128256 bf16 185 us, one element off 569; policy 227 / 496, 1800 x 128256 fp32 356 / 405.
 constexpr int DEPTH = 4;   // rows whose sums may be on their way
 
 struct alignas(16) Control {
