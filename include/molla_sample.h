@@ -436,9 +436,9 @@ int32_t molla_sample_token_logprobs_backward(const void *d_logits, int32_t logit
                                              int64_t grad_stride);
 
 /* The same with one more value a row between them, for losses with an entropy term: d_depth [B] (NULL = not wanted) is sum p (max z - z), how
- * far the entropy lies above ln of the stats' sum. The backward form takes it in place of the entropy, which at 12 nats is
- * rounded to 5e-7: in rows of logits close to one another, whose depth is a tenth, that is all but the gradient's fifth digit.
- * With it the gradient is, bit for bit, that of the policy loss for the same derivatives. */
+ * far the entropy lies above ln of the stats' sum. The backward form takes it in place of the entropy, which at 12 nats is rounded
+ * to 5e-7: in rows of logits close to one another, whose depth is a tenth, that is in the fifth digit of the entropy's gradient.
+ * With the depth the gradient is, bit for bit, that of the policy loss for the same derivatives. */
 int32_t molla_sample_token_logprobs_with_depth(const void *d_logits, int32_t logits_type, int64_t row_stride, int32_t B,
                                                int32_t V, const int32_t *d_tokens, const float *d_temperature, void *stream,
                                                float *d_logprob, float *d_entropy, float *d_depth, float *d_stats,
